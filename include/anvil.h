@@ -197,7 +197,10 @@ int anvil_mmvq_glu_f32(int ggml_type, const void *W_gate, const void *W_up, cons
 /* Reads and clears the device status words of the current device: the OR of
  * anvil_device_status flags set by kernels whose bounded waits gave up (0 = none),
  * or a negative anvil_status.  Synchronous. */
-enum anvil_device_status { ANVIL_DEVICE_MBAR_TIMEOUT = 1 };
+enum anvil_device_status {
+    ANVIL_DEVICE_MBAR_TIMEOUT = 1,
+    ANVIL_DEVICE_BAD_PAGE = 2 /* the cache's operators met a page number, start or length out of range */
+};
 int anvil_take_device_status(void);
 
 /* Parity probe: runs the production MMVQ kernel with its integer block sums written
@@ -369,6 +372,73 @@ int anvil_ipc_alloc(size_t bytes, void **ptr, void *handle);
 int anvil_ipc_open(const void *handle, void **ptr);
 int anvil_ipc_close(void *ptr);
 int anvil_ipc_free(void *ptr);
+
+/* ---- paged key/value cache and attention over it -------------------------- */
+
+/* The part of a decoder between its k/v products and its output product: the cache that the
+ * new keys and values go into, and the attention that reads it.  No counterpart in the
+ * reference (llama.cpp runs it between the mul_mat_vec_q launches that the reference tunes,
+ * docs/decode-pipeline-breakdown.md:20-21).
+ *
+ * A cache holds one layer: k and v are (num_pages, kv_heads, page_size, row), row-major, where a
+ * row is head_dim values of `kind` (ggml type ids):
+ *   1 F16, 30 BF16: 16-bit values; k_scale = v_scale = NULL.
+ *   8 Q8_0: int8 codes.  2 Q4_0: head_dim / 2 bytes, nibbles in GGUF order (value e < 16 of
+ *   a 32-value block in the low nibble of its byte e, e >= 16 in the high nibble of byte
+ *   e - 16; nibble - 8).  The scales (fp16, one per 32 values) are k_scale and v_scale,
+ *   (num_pages, kv_heads, page_size, head_dim / 32).
+ * head_dim 64, 128 or 256; page_size a power of two, 1..1024; all tensors 16-byte aligned. */
+typedef struct anvil_kv_cache {
+    int kind, num_pages, kv_heads, page_size, head_dim;
+    void *k, *v, *k_scale, *v_scale;
+} anvil_kv_cache;
+
+/* A ragged batch on the device.  Sequence b has the packed rows start[b] .. start[b+1]-1 of the
+ * call's k, v, q and out (start: batch + 1 values, ascending); rows behind start[batch] (of
+ * `total`) are neither read nor written.  kv_len[b] tokens of it are in the cache, the new ones
+ * included: its row i is at position kv_len[b] - (start[b+1] - start[b]) + i.  Position p is in
+ * page page_table[b * page_table_stride + p / page_size].  Entries are read on the device: one
+ * that is out of range is cut or skipped, never followed, and raises ANVIL_DEVICE_BAD_PAGE. */
+typedef struct anvil_kv_batch {
+    const int32_t *page_table;
+    int64_t page_table_stride;
+    int max_pages, batch, total;
+    const int32_t *start, *kv_len;
+} anvil_kv_batch;
+
+/* Puts the new rows' keys and values at their positions.  dtype of k and v: 0 F32, 1 F16,
+ * 30 BF16; row and head strides in values, rows of head_dim contiguous values starting on
+ * 16-byte boundaries.  Quantised kinds, per 32 values with largest magnitude M, by exact
+ * arithmetic: Q8_0 code = 127 x / M to the nearest integer, halves away from zero, scale
+ * fp16(M / 127); Q4_0 with d = -top / 8 (top: the value of magnitude M, the first of equals)
+ * nibble = min(15, floor(x / d + 8.5)), scale fp16(d): the GGUF types' rules.  Magnitudes
+ * above 65024 (infinity too) are stored as 65024 there; a block with a NaN reads back as NaN.
+ * Two rows at one position: either may win. */
+int anvil_kv_write(const anvil_kv_cache *cache, const anvil_kv_batch *batch, int dtype, const void *k,
+                   int64_t k_row_stride, int64_t k_head_stride, const void *v, int64_t v_row_stride,
+                   int64_t v_head_stride, anvil_stream_t stream);
+
+/* The cached values of positions first[b] + i (first NULL: i) for the packed rows of each
+ * sequence (batch->kv_len is not read), as (total, kv_heads, head_dim) of dtype 0, 1 or 30,
+ * each code * scale rounded once; zeros for a position without a page. */
+int anvil_kv_read(const anvil_kv_cache *cache, const anvil_kv_batch *batch, const int32_t *first, int dtype,
+                  void *k, void *v, anvil_stream_t stream);
+
+/* out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j over the cached tokens j that the row
+ * sees: all kv_len[b] of its sequence, or, causal, those up to its own position; zeros for a
+ * row that sees none.  Query head h reads key/value head h / (heads / kv_heads).  q: dtype 1
+ * or 30, for an F16 / BF16 cache the cache's own; strides in values, 16-byte aligned rows; out:
+ * (total, heads, head_dim), contiguous, of q's type.  Keys without a page are left out.  What
+ * lies behind kv_len in a page is never used; keys that a row does not see do not reach it, NaN
+ * and infinities among them.  Products run on the tensor cores in fp16 (F16 and quantised caches)
+ * or bf16, with fp32 sums; q of a quantised cache is scaled by a power of two into
+ * fp16's range.  workspace: anvil_paged_attention_workspace(cache, batch, heads) bytes of
+ * scratch for this call (it depends on batch, total, max_pages and heads alone, not on the
+ * lengths), 16-byte aligned; calls that may overlap need their own. */
+int64_t anvil_paged_attention_workspace(const anvil_kv_cache *cache, const anvil_kv_batch *batch, int heads);
+int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv_batch *batch, int dtype, const void *q,
+                          int64_t q_row_stride, int64_t q_head_stride, int heads, float scale, int causal,
+                          void *out, void *workspace, int64_t workspace_bytes, anvil_stream_t stream);
 
 /* ---- smithy runtime config (replaces patches/smithy-config.h) ------------ */
 

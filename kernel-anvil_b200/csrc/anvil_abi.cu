@@ -237,6 +237,8 @@ MmvqKernelFn mmvq_mma_kernel_for(int qt, int ncols, int mode);
 int mmvq_mma_smem_bytes(int qt, int K, int ncols, int nwarps, int nstages);
 int mmvq_mma_max_warps();
 int mmvq_mma_take_status();
+int kv_take_status();
+int attn_take_status();
 constexpr int kMmaTileRows = 16;
 // Smallest column count that takes the tensor-core path (0: never).
 // 4: at 2 columns the MMA tiles compute 8 columns' work and the dp4a kernels are faster
@@ -846,7 +848,7 @@ int anvil_mmvq_block_sums(int ggml_type, const void *W, const void *xq, int32_t 
 // flags (0 = no bounded wait gave up) or a negative status.
 int anvil_take_device_status(void) {
     int v = 0;
-    int parts[21] = {take_quantize_status(), mmvq_mma_take_status(), mmvq_kernel_q4k_take_status(),
+    int parts[23] = {kv_take_status(), attn_take_status(), take_quantize_status(), mmvq_mma_take_status(), mmvq_kernel_q4k_take_status(),
                     mmvq_kernel_q5k_take_status(), mmvq_kernel_q6k_take_status(),
                     mmvq_kernel_q80_take_status(), mmvq_kernel_q40_take_status(),
                     mmvq_kernel_q41_take_status(), mmvq_kernel_q50_take_status(),

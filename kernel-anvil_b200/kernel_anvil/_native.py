@@ -224,6 +224,12 @@ SIGNATURES = {
     "anvil_ipc_open": (c_int, [c_void_p, ctypes.POINTER(c_void_p)]),
     "anvil_ipc_close": (c_int, [c_void_p]),
     "anvil_ipc_free": (c_int, [c_void_p]),
+    "anvil_kv_write": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+                               c_int64, c_void_p]),
+    "anvil_kv_read": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "anvil_paged_attention_workspace": (c_int64, [c_void_p, c_void_p, c_int]),
+    "anvil_paged_attention": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int,
+                                      ctypes.c_float, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
     "anvil_smithy_bucket": (c_int, [c_int]),
     "anvil_smithy_set_model": (None, [c_char_p]),
     "anvil_smithy_load": (c_int, [c_char_p]),
