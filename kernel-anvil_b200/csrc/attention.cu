@@ -15,9 +15,8 @@ namespace anvil {
 
 int kv_check(const anvil_kv_cache *c, const anvil_kv_batch *b, KvCacheView *cv, KvBatchView *bv);
 
-int attn_rows_ctas_per_sm(int kind, int D);
-int64_t attn_rows_part_bytes(int D);
-int attn_rows_launch(int kind, int D, const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
+AttnTiles attn_rows_tiles(int kind, int D, int nt);
+int attn_rows_launch(int kind, int D, int nt, const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
                      bool join, cudaStream_t s);
 int attn_rows_take_status();
 
@@ -26,21 +25,24 @@ int attn_take_status() { return attn_rows_take_status(); }
 // The grid: every resident slot, or fewer where the batch cannot have that many key tiles.  It
 // follows from the batch's outer sizes, not from lengths, which are on the device.
 struct AttnPlan {
+    int nt;         // row tile in eighths
     int ctas;
     bool join;      // some unit may span CTAs
     int64_t bytes;  // of partial results
 };
 
 static AttnPlan attn_plan(const anvil_kv_cache *c, const KvCacheView &cv, const KvBatchView &bv, int heads) {
-    const int group = heads / cv.kv_heads, rows = 16, keys = 64;
-    const int64_t capacity = std::min<int64_t>(int64_t(bv.max_pages) << cv.page_shift, 0x7fffffff);
-    const int64_t units = int64_t(cv.kv_heads) * (int64_t(bv.total) * group / rows + std::min(bv.batch, bv.total));
-    const int64_t per = std::max<int64_t>(1, (capacity + keys - 1) / keys);
-    const int64_t slots = 148 * attn_rows_ctas_per_sm(c->kind, c->head_dim);
+    const int group = heads / cv.kv_heads;
     AttnPlan p;
+    p.nt = int64_t(bv.total) * group <= int64_t(bv.batch) * 8 ? 1 : 2;
+    const AttnTiles t = attn_rows_tiles(c->kind, c->head_dim, p.nt);
+    const int64_t capacity = std::min<int64_t>(int64_t(bv.max_pages) << cv.page_shift, 0x7fffffff);
+    const int64_t units = int64_t(cv.kv_heads) * (int64_t(bv.total) * group / t.rows + std::min(bv.batch, bv.total));
+    const int64_t per = std::max<int64_t>(1, (capacity + t.keys - 1) / t.keys);
+    const int64_t slots = 148 * t.occ;
     p.ctas = int(per > slots / std::max<int64_t>(units, 1) ? slots : std::min(slots, units * per));
     p.join = per > 1;
-    p.bytes = p.join ? attn_rows_part_bytes(c->head_dim) * p.ctas : 0;
+    p.bytes = p.join ? int64_t(t.rows) * (c->head_dim + 2) * 8 * p.ctas : 0;
     return p;
 }
 
@@ -83,6 +85,6 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
                     (long long)(workspace ? workspace_bytes : 0));
     const AttnIO io{q, q_row_stride, q_head_stride, out, heads, heads / cv.kv_heads, scale * 1.4426950408889634f,
                     causal != 0, dtype == kKvBF16, static_cast<float *>(workspace)};
-    return attn_rows_launch(cache->kind, cache->head_dim, cv, bv, io, p.ctas, p.join,
+    return attn_rows_launch(cache->kind, cache->head_dim, p.nt, cv, bv, io, p.ctas, p.join,
                             reinterpret_cast<cudaStream_t>(stream));
 }

@@ -14,6 +14,8 @@
 
 #include <cuda_runtime.h>
 
+#include "anvil.h"
+#include "anvil_host.h"
 #include "kv_cache.cuh"
 
 namespace anvil {
@@ -259,6 +261,27 @@ __global__ void __launch_bounds__(128) attn_join_kernel(KvCacheView c, KvBatchVi
         out[at] = io.q_bf16 ? pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv)
                             : pack_half(o[2 * j] * inv, o[2 * j + 1] * inv);
     }
+}
+
+// Host side: a kernel's row tile, key tile and resident CTAs of an SM.
+struct AttnTiles {
+    int rows, keys, occ;
+};
+
+template <int ROWS, int KEYS, int D>
+static int attn_join_launch(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
+                            cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas, ROWS / 4);
+    cfg.blockDim = 128;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_join_kernel<ROWS, KEYS, D>, c, bt, io);
+    return e == cudaSuccess ? ANVIL_OK : cuda_fail(e, "paged_attention join launch");
 }
 
 }  // namespace anvil
