@@ -9,10 +9,11 @@
 // it works a fifth of the time at the rate at which HBM delivers keys, and tcgen05's smallest tile
 // has 64 rows, of which a decode step fills 8.
 //
-// Loads: each warp owns a ring of stages of 16 keys.  Lane r copies the row of key r (lanes 16..31:
-// of its value) with one bulk copy through the page table, so pages of any size look alike and no
-// lane computes addresses for another; the scales follow by cp.async.  Rows are padded by 16 bytes,
-// which makes the reads below free of bank conflicts.  Codes are widened straight from the ring into
+// Loads: each warp owns a ring of stages of 16 keys, filled by cp.async.  Pages of 16 keys and more
+// hold whole steps, whose rows are one run of memory; in smaller pages each key's row is looked up
+// and handed to the lanes that copy it.  (One bulk copy a row was tried: the instruction takes
+// uniform operands, so 32 of them become a loop of 400 instructions a step.)  Rows are padded by 16
+// bytes, which makes the reads below free of bank conflicts.  Codes are widened straight from the ring into
 // MMA operands: the order of a product's inner dimension is free as long as both operands share it,
 // so a lane feeds the contiguous values of its key to consecutive MMAs, and the query's operands
 // are gathered to match once; the same holds for the order of the head's dimensions in O^T, which
@@ -64,6 +65,11 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Copies 16 bytes to shared memory, of which the first n are read and the others zero.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
 // Transposes an 8 x 8 matrix of 16-bit values held two to a lane.
@@ -133,7 +139,7 @@ template <int KIND, int D> __device__ __forceinline__ int v_dim(int i, int g) {
 
 template <int KIND, int D, int NT>
 __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_ctas)
-    attn_rows_kernel(KvCacheView c, KvBatchView bt, AttnIO io, uint64_t limit_ns) {
+    attn_rows_kernel(KvCacheView c, KvBatchView bt, AttnIO io) {
     using S = RowsShape<KIND, D, NT>;
     constexpr int ROWS = S::rows;
     constexpr int NS = D / 16;   // QK steps
@@ -141,13 +147,10 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
     constexpr bool BF = S::bf16;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ AttnScratch sc;
-    __shared__ uint64_t bars[kRowsWarps][4];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cq = lane & 3;
     uint8_t *ring = smem + warp * S::per_warp;
-    uint64_t *bar = bars[warp];
-    if (lane < S::stages) mbar_init(&bar[lane], 1);
-    mbar_fence_init();
+    const bool whole = c.page_shift >= 4;
 
     const int64_t work = attn_locate<ROWS, kRowsKeys>(
         c, bt, io, &sc,
@@ -162,7 +165,6 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
     const int64_t lo = attn_share(work, blockIdx.x, ctas), hi = attn_share(work, blockIdx.x + 1, ctas);
     AttnPos p = sc.pos;
     int slot = 0, fill = 0;     // ring slots: next to be worked on, next to be filled
-    uint32_t phase = 0;         // bit per slot: parity of its next completion
 
     while (p.b < bt.batch && p.unit0 < hi) {
         const AttnSeq<ROWS, kRowsKeys> q(load_seq(bt, c, p.b), io);
@@ -173,39 +175,63 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
 
         // ---- the ring: step s covers keys 16 s .. 16 s + 15
         const int step0 = t0 * 4 + warp, steps = (key_end + kRowsStep - 1) / kRowsStep;
-        auto row_of = [&](int s) -> int64_t {  // cache row of key 16 s + lane % 16; -1: no page, -2: no key
-            const int key = s * kRowsStep + (lane & 15);
+        // Cache row of key 16 s + lane % 16 (-1: no page, -2: no key); where pages hold 16 keys and more, and so
+        // whole steps, the row of key 16 s on every lane.
+        auto row_of = [&](int s) -> int64_t {
+            const int key = s * kRowsStep + (whole ? 0 : lane & 15);
             if (s >= steps || key >= key_end) return -2;
             return kv_lookup(bt, c, p.b, key, p.head);
         };
         auto issue = [&](int s, int64_t row) {
             if (s < steps) {
                 uint8_t *st = ring + fill * S::stage;
-                const uint32_t live = __ballot_sync(0xffffffffu, row >= 0);
-                const uint32_t bad = __ballot_sync(0xffffffffu, row == -1) & 0xFFFFu;
-                uint8_t *dst = lane < 16 ? st + lane * S::kst : st + S::off_v + (lane - 16) * S::vst;
-                if (live != 0xffffffffu && row < 0) {  // keys that are not there: zeros
+                const uint32_t dst = smem_u32(st) + (lane / S::ch) * S::kst + (lane % S::ch) * 16;
+                const uint32_t dst_v = smem_u32(st) + S::off_v + (lane / S::ch) * S::vst + (lane % S::ch) * 16;
+                uint32_t bad;
+                if (whole) {
+                    const int live = row < 0 ? 0 : min(kRowsStep, key_end - s * kRowsStep);
+                    bad = row == -1 ? 0xFFFFu : 0;
+                    const int64_t off = max(row, int64_t(0)) * S::rb + lane * 16;
 #pragma unroll
-                    for (int i = 0; i < S::ch; ++i) reinterpret_cast<uint4 *>(dst)[i] = make_uint4(0, 0, 0, 0);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the slot's next copy
+                    for (int j = 0; j < S::ch / 2; ++j) {
+                        const int n = lane / S::ch + j * (32 / S::ch) < live ? 16 : 0;  // 0: zeros are written
+                        cp_async16(dst + j * (32 / S::ch) * S::kst, c.k + off + j * 512, n);
+                        cp_async16(dst_v + j * (32 / S::ch) * S::vst, c.v + off + j * 512, n);
+                    }
+                    if constexpr (S::quant) {  // 16 rows' scales: sb chunks of 16 bytes of each tensor
+                        if (lane < 2 * S::sb) {
+                            const int i = lane & (S::sb - 1);
+                            const uint8_t *src = reinterpret_cast<const uint8_t *>(lane < S::sb ? c.ks : c.vs);
+                            // (a chunk of scales may cover rows behind the last: bytes, not chunks, are cut)
+                            const int n = max(0, min(16, live * S::sb - i * 16));
+                            cp_async16(smem_u32(st) + S::off_s + lane * 16,
+                                       src + max(row, int64_t(0)) * S::sb + i * 16, n);
+                        }
+                    }
+                } else {
+                    bad = __ballot_sync(0xffffffffu, row == -1) & 0xFFFFu;
+#pragma unroll
+                    for (int j = 0; j < S::ch / 2; ++j) {
+                        const int64_t rw = __shfl_sync(0xffffffffu, row, lane / S::ch + j * (32 / S::ch));
+                        const int64_t off = max(rw, int64_t(0)) * S::rb + (lane % S::ch) * 16;
+                        cp_async16(dst + j * (32 / S::ch) * S::kst, c.k + off, rw < 0 ? 0 : 16);
+                        cp_async16(dst_v + j * (32 / S::ch) * S::vst, c.v + off, rw < 0 ? 0 : 16);
+                    }
+                    if constexpr (S::quant) {
+                        const uint8_t *src = reinterpret_cast<const uint8_t *>(lane < 16 ? c.ks : c.vs);
+                        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(
+                                         smem_u32(st) + S::off_s + lane * S::sb),
+                                     "l"(src + max(row, int64_t(0)) * S::sb), "n"(S::sb), "r"(row < 0 ? 0 : S::sb)
+                                     : "memory");
+                    }
                 }
                 if (lane == 0) {
                     *reinterpret_cast<uint32_t *>(st + S::off_bad) = bad;
                     if (bad) flag_bad_page();
-                    mbar_arrive_expect_tx(&bar[fill], __popc(live) * S::rb);
-                }
-                __syncwarp();
-                if (row >= 0) bulk_copy_g2s(dst, (lane < 16 ? c.k : c.v) + row * S::rb, S::rb, &bar[fill]);
-                if constexpr (S::quant) {
-                    const uint8_t *src = reinterpret_cast<const uint8_t *>(lane < 16 ? c.ks : c.vs);
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(
-                                     smem_u32(st + S::off_s + lane * S::sb)),
-                                 "l"(src + (row < 0 ? 0 : row * S::sb)), "n"(S::sb), "r"(row < 0 ? 0 : S::sb)
-                                 : "memory");
                 }
                 if (++fill == S::stages) fill = 0;
             }
-            if constexpr (S::quant) asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
 
         int64_t next = row_of(step0);
@@ -290,9 +316,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                 __syncwarp();
                 issue(s + 4 * (S::stages - 1), row);
             }
-            if constexpr (S::quant) asm volatile("cp.async.wait_group %0;" ::"n"(S::stages - 1) : "memory");
-            mbar_wait_bounded(&bar[slot], (phase >> slot) & 1, limit_ns);
-            phase ^= 1u << slot;
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::stages - 1) : "memory");
             __syncwarp();
             uint8_t *sk = ring + slot * S::stage, *sv = sk + S::off_v;
             __half *ks = reinterpret_cast<__half *>(sk + S::off_s);
@@ -457,7 +481,6 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                             *w &= ~nonfinite2<BF>(*w);
                         }
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the slot's next copy
                     __syncwarp();
                 }
             }
@@ -547,7 +570,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
             }
             if (++slot == S::stages) slot = 0;
         }
-        if constexpr (S::quant) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
 
         // ---- join the four warps: maxima and sums, then the outputs by rows
 #pragma unroll
@@ -615,9 +638,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                 part[ROWS * D + ROWS + r] = sum;
             }
         }
-        // the rings were written by plain stores; the copies that come next are of another proxy
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
+        __syncthreads();  // before the rings are filled again
         attn_next(c, bt, io, p, q);
     }
 }
@@ -636,7 +657,7 @@ template <int KIND, int D, int NT> struct RowsOps {
         cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<KIND, D, NT>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
-        attn_rows_kernel<KIND, D, NT><<<ctas, kRowsWarps * 32, S::smem, stream>>>(c, bt, io, wait_limit_ns());
+        attn_rows_kernel<KIND, D, NT><<<ctas, kRowsWarps * 32, S::smem, stream>>>(c, bt, io);
         if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "paged_attention launch");
         return join ? attn_join_launch<S::rows, kRowsKeys, D>(c, bt, io, ctas, stream) : ANVIL_OK;
     }
