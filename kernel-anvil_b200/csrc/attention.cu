@@ -6,6 +6,7 @@
 //   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  m = max_j s_j;  o = 0 where nothing is seen.
 // Keys are visited once with a running maximum and sum (fp32).
 #include <algorithm>
+#include <cmath>
 
 #include "anvil.h"
 #include "anvil_host.h"
@@ -19,13 +20,20 @@ AttnTiles attn_rows_tiles(int kind, int D, int nt);
 int attn_rows_launch(int kind, int D, int nt, const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
                      bool join, cudaStream_t s);
 int attn_rows_take_status();
+AttnTiles attn_tile_tiles(int D);
+int attn_tile_launch(int kind, int D, const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas, bool join,
+                     cudaStream_t s);
+int attn_tile_take_status();
 
-int attn_take_status() { return attn_rows_take_status(); }
+int attn_take_status() {
+    const int a = attn_rows_take_status(), b = attn_tile_take_status();
+    return a < 0 ? a : b < 0 ? b : a | b;
+}
 
 // The grid: every resident slot, or fewer where the batch cannot have that many key tiles.  It
 // follows from the batch's outer sizes, not from lengths, which are on the device.
 struct AttnPlan {
-    int nt;         // row tile in eighths
+    int nt;         // row tile of the rows kernel in eighths; 0: the tile kernel
     int ctas;
     bool join;      // some unit may span CTAs
     int64_t bytes;  // of partial results
@@ -34,8 +42,9 @@ struct AttnPlan {
 static AttnPlan attn_plan(const anvil_kv_cache *c, const KvCacheView &cv, const KvBatchView &bv, int heads) {
     const int group = heads / cv.kv_heads;
     AttnPlan p;
-    p.nt = int64_t(bv.total) * group <= int64_t(bv.batch) * 8 ? 1 : 2;
-    const AttnTiles t = attn_rows_tiles(c->kind, c->head_dim, p.nt);
+    const int64_t rows = int64_t(bv.total) * group;
+    p.nt = rows <= int64_t(bv.batch) * 8 ? 1 : rows <= int64_t(bv.batch) * 16 ? 2 : 0;
+    const AttnTiles t = p.nt ? attn_rows_tiles(c->kind, c->head_dim, p.nt) : attn_tile_tiles(c->head_dim);
     const int64_t capacity = std::min<int64_t>(int64_t(bv.max_pages) << cv.page_shift, 0x7fffffff);
     const int64_t units = int64_t(cv.kv_heads) * (int64_t(bv.total) * group / t.rows + std::min(bv.batch, bv.total));
     const int64_t per = std::max<int64_t>(1, (capacity + t.keys - 1) / t.keys);
@@ -76,6 +85,7 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
         return fail(ANVIL_ERR_INVALID, "heads=%d is not a multiple of kv_heads=%d", heads, cv.kv_heads);
     if (bv.batch == 0 || bv.total == 0) return ANVIL_OK;
     if (!q || !out || !bv.kv_len) return fail(ANVIL_ERR_INVALID, "null q, out or kv_len");
+    if (!std::isfinite(scale)) return fail(ANVIL_ERR_INVALID, "scale=%f is not finite", double(scale));
     const auto mis = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
     if (mis(q) || mis(out) || mis(workspace) || q_row_stride % 8 || q_head_stride % 8)
         return fail(ANVIL_ERR_ALIGN, "q, its rows, out and the workspace must be 16-byte aligned");
@@ -85,6 +95,9 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
                     (long long)(workspace ? workspace_bytes : 0));
     const AttnIO io{q, q_row_stride, q_head_stride, out, heads, heads / cv.kv_heads, scale * 1.4426950408889634f,
                     causal != 0, dtype == kKvBF16, static_cast<float *>(workspace)};
+    if (!p.nt)
+        return attn_tile_launch(cache->kind, cache->head_dim, cv, bv, io, p.ctas, p.join,
+                                reinterpret_cast<cudaStream_t>(stream));
     return attn_rows_launch(cache->kind, cache->head_dim, p.nt, cv, bv, io, p.ctas, p.join,
                             reinterpret_cast<cudaStream_t>(stream));
 }

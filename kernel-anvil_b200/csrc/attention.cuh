@@ -14,6 +14,8 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "anvil.h"
 #include "anvil_host.h"
 #include "kv_cache.cuh"
@@ -199,8 +201,41 @@ template <bool BF16> __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) 
     return ((w & E) == E ? 0xFFFFu : 0u) | (((w >> 16) & E) == E ? 0xFFFF0000u : 0u);
 }
 
+// Value e of a cache row.
+template <int KIND, int D>
+__device__ __forceinline__ float kv_value(const uint8_t *data, const __half *scales, int64_t row, int e) {
+    if constexpr (KIND == kKvF16) {
+        return __half2float(reinterpret_cast<const __half *>(data)[row * D + e]);
+    } else if constexpr (KIND == kKvBF16) {
+        return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(data)[row * D + e]);
+    } else if constexpr (KIND == kKvQ8_0) {
+        return float(reinterpret_cast<const int8_t *>(data)[row * D + e]) *
+               __half2float(scales[row * (D / 32) + e / 32]);
+    } else {
+        const uint8_t w = data[row * (D / 2) + (e / 32) * 16 + (e % 16)];
+        return float(int((e % 32) < 16 ? w & 15 : w >> 4) - 8) * __half2float(scales[row * (D / 32) + e / 32]);
+    }
+}
+
+__device__ __forceinline__ uint32_t h2sub(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2mul(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t dup16(uint32_t x) { return __byte_perm(x, x, 0x1010); }
+
 // Joins the partial results of the unit that CTA `blockIdx.x` of the attention kernel began and did
-// not finish, 4 rows of it (blockIdx.y): o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.
+// not finish, every gridDim.y-th four rows of it: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.
 template <int ROWS, int KEYS, int D>
 __global__ void __launch_bounds__(128) attn_join_kernel(KvCacheView c, KvBatchView bt, AttnIO io) {
     __shared__ AttnScratch sc;
@@ -222,44 +257,46 @@ __global__ void __launch_bounds__(128) attn_join_kernel(KvCacheView c, KvBatchVi
     const int64_t end = p.unit0 + q.key_tiles(p.mt);
     if (end <= hi) return;  // finished where it was begun
     const int last = attn_owner(work, end - 1, ctas);
-    const int row = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int64_t r = int64_t(p.mt) * ROWS + row;
-    if (row >= ROWS || r >= int64_t(q.n) * q.group) return;
+    const int lane = threadIdx.x & 31;
     using P = AttnPart<ROWS, D>;
-    float m = -INFINITY;
-    for (int i = cta + lane; i <= last; i += 32) m = fmaxf(m, P::slot(io.part, i, i == cta)[ROWS * D + row]);
-    m = warp_max(m);
-    const float base = m == -INFINITY ? 0.0f : m;
-    constexpr int V = D / 32;
-    float o[V] = {}, l = 0.0f;
-    for (int i = cta; i <= last; ++i) {
-        const float *s = P::slot(io.part, i, i == cta);
-        const float a = ex2(s[ROWS * D + row] - base);
-        l += a * s[ROWS * D + ROWS + row];
-        if constexpr (V == 2) {
-            const float2 x = *reinterpret_cast<const float2 *>(s + row * D + lane * 2);
-            o[0] += a * x.x;
-            o[1] += a * x.y;
-        } else {
+    for (int row = blockIdx.y * 4 + (threadIdx.x >> 5); row < ROWS; row += 4 * gridDim.y) {
+        const int64_t r = int64_t(p.mt) * ROWS + row;
+        if (r >= int64_t(q.n) * q.group) return;
+        float m = -INFINITY;
+        for (int i = cta + lane; i <= last; i += 32) m = fmaxf(m, P::slot(io.part, i, i == cta)[ROWS * D + row]);
+        m = warp_max(m);
+        const float base = m == -INFINITY ? 0.0f : m;
+        constexpr int V = D / 32;
+        float o[V] = {}, l = 0.0f;
+        for (int i = cta; i <= last; ++i) {
+            const float *s = P::slot(io.part, i, i == cta);
+            const float a = ex2(s[ROWS * D + row] - base);
+            l += a * s[ROWS * D + ROWS + row];
+            if constexpr (V == 2) {
+                const float2 x = *reinterpret_cast<const float2 *>(s + row * D + lane * 2);
+                o[0] += a * x.x;
+                o[1] += a * x.y;
+            } else {
 #pragma unroll
-            for (int j = 0; j < V / 4; ++j) {
-                const float4 x = *reinterpret_cast<const float4 *>(s + row * D + j * 128 + lane * 4);
-                o[4 * j] += a * x.x;
-                o[4 * j + 1] += a * x.y;
-                o[4 * j + 2] += a * x.z;
-                o[4 * j + 3] += a * x.w;
+                for (int j = 0; j < V / 4; ++j) {
+                    const float4 x = *reinterpret_cast<const float4 *>(s + row * D + j * 128 + lane * 4);
+                    o[4 * j] += a * x.x;
+                    o[4 * j + 1] += a * x.y;
+                    o[4 * j + 2] += a * x.z;
+                    o[4 * j + 3] += a * x.w;
+                }
             }
         }
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int token = q.s.q0 + int(r / q.group), h = p.head * q.group + int(r % q.group);
-    uint32_t *out = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(io.out) +
-                                                 (int64_t(token) * io.heads + h) * D);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int token = q.s.q0 + int(r / q.group), h = p.head * q.group + int(r % q.group);
+        uint32_t *out = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(io.out) +
+                                                     (int64_t(token) * io.heads + h) * D);
 #pragma unroll
-    for (int j = 0; j < V / 2; ++j) {
-        const int at = V == 2 ? lane : (j / 2) * 64 + lane * 2 + (j & 1);
-        out[at] = io.q_bf16 ? pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv)
-                            : pack_half(o[2 * j] * inv, o[2 * j + 1] * inv);
+        for (int j = 0; j < V / 2; ++j) {
+            const int at = V == 2 ? lane : (j / 2) * 64 + lane * 2 + (j & 1);
+            out[at] = io.q_bf16 ? pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv)
+                                : pack_half(o[2 * j] * inv, o[2 * j + 1] * inv);
+        }
     }
 }
 
@@ -272,7 +309,7 @@ template <int ROWS, int KEYS, int D>
 static int attn_join_launch(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
                             cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, ROWS / 4);
+    cfg.gridDim = dim3(ctas, std::min(ROWS / 4, 8));
     cfg.blockDim = 128;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

@@ -79,23 +79,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     return r;
 }
 
-__device__ __forceinline__ uint32_t h2sub(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t h2mul(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t h2fma(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t r;
-    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
-__device__ __forceinline__ uint32_t dup16(uint32_t x) { return __byte_perm(x, x, 0x1010); }
-
 // Codes to fp16 pairs: a byte or nibble below the exponent of 1024 (or 16 times a nibble) is an fp16
 // number that differs from the code by a constant, taken off exactly.
 __device__ __forceinline__ uint32_t q8_pair(uint32_t u, uint32_t sel) {  // bytes are code + 128
