@@ -83,6 +83,8 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
         return fail(ANVIL_ERR_UNSUPPORTED, "an unquantised cache takes q of its own type");
     if (heads < 1 || heads % cv.kv_heads)
         return fail(ANVIL_ERR_INVALID, "heads=%d is not a multiple of kv_heads=%d", heads, cv.kv_heads);
+    if (int64_t(bv.total) * heads > 0x7fffffff - 1024)
+        return fail(ANVIL_ERR_UNSUPPORTED, "%d rows of %d heads are too many for one call", bv.total, heads);
     if (bv.batch == 0 || bv.total == 0) return ANVIL_OK;
     if (!q || !out || !bv.kv_len) return fail(ANVIL_ERR_INVALID, "null q, out or kv_len");
     if (!std::isfinite(scale)) return fail(ANVIL_ERR_INVALID, "scale=%f is not finite", double(scale));

@@ -42,124 +42,192 @@ template <int ROWS, int D> struct AttnPart {
     }
 };
 
-// One sequence's units: row tiles and their key tiles.
+// One sequence's units: row tiles and their key tiles.  Rows are counted in 32 bits (the host refuses
+// batches of 2^31 query rows).
 template <int ROWS, int KEYS> struct AttnSeq {
     KvSeq s;
     int n, group, causal, tiles;  // new tokens; row tiles
 
     __device__ __forceinline__ AttnSeq(const KvSeq &seq, const AttnIO &io)
         : s(seq), n(seq.q1 - seq.q0), group(io.group), causal(io.causal),
-          tiles(int((int64_t(n) * io.group + ROWS - 1) / ROWS)) {}
+          tiles(int((unsigned(n) * unsigned(io.group) + ROWS - 1) / ROWS)) {}
 
     // Keys that some row of tile mt sees (its last token's), and their key tiles: at least one,
     // so that rows without keys are visited and get their zeros.
     __device__ __forceinline__ int keys(int mt) const {
-        const int last = min(n - 1, int((int64_t(mt + 1) * ROWS - 1) / group));
-        return kv_seen(last, n, s.kv, causal);
+        if (!causal) return s.kv;
+        const int last = min(n - 1, int((unsigned(mt + 1) * ROWS - 1) / unsigned(group)));
+        return kv_seen(last, n, s.kv, true);
     }
     __device__ __forceinline__ int key_tiles(int mt) const { return max(1, (keys(mt) + KEYS - 1) / KEYS); }
-    __device__ __forceinline__ int64_t head_work() const {  // key tiles of one head
-        if (!causal) return int64_t(tiles) * key_tiles(0);
-        int64_t w = 0;
-        for (int mt = 0; mt < tiles; ++mt) w += key_tiles(mt);
-        return w;
+};
+
+// A place in the order of all key tiles.  A unit counts COST places before its first key tile, what it
+// takes to begin and end one in terms of a key tile's time.
+struct AttnPos {
+    int b, head, mt;
+    int64_t unit0;  // place of the unit's first key tile
+};
+
+// a / b without the long 64-bit division where both are short
+__device__ __forceinline__ int64_t div64(int64_t a, int64_t b) {
+    return (a | b) >> 32 ? a / b : int64_t(unsigned(a) / unsigned(b));
+}
+
+// The division of `work` places over the grid: the first `more` CTAs get per + 1, the others per.
+// CTAs that work: each has at least one place.
+struct AttnShares {
+    int64_t per;
+    int ctas, more;
+    __device__ __forceinline__ AttnShares(int64_t work, int grid) {
+        ctas = int(min(work, int64_t(grid)));
+        per = ctas ? div64(work, ctas) : 0;
+        more = int(work - per * ctas);
+    }
+    __device__ __forceinline__ int64_t begin(int c) const { return per * c + min(c, more); }
+    __device__ __forceinline__ int owner(int64_t place) const {  // the CTA whose share holds it
+        const int64_t cut = (per + 1) * more;
+        return place < cut ? int(div64(place, per + 1)) : more + int(div64(place - cut, per));
     }
 };
 
-// A place in the order of all key tiles.
-struct AttnPos {
-    int b, head, mt, tile;  // key tile `tile` of the unit
-    int64_t unit0;          // global number of the unit's first key tile
-};
-
-// CTAs that work: each has at least one key tile.
-__device__ __forceinline__ int attn_ctas(int64_t work, int grid) { return int(min(work, int64_t(grid))); }
-// CTA c's share of `work` key tiles is [share(c), share(c + 1)).
-__device__ __forceinline__ int64_t attn_share(int64_t work, int c, int ctas) { return work * c / ctas; }
-// The CTA whose share holds key tile t: the last c with share(c) <= t.
-__device__ __forceinline__ int attn_owner(int64_t work, int64_t t, int ctas) {
-    return int(((t + 1) * ctas - 1) / work);
-}
-
-// All threads: the total work, and the position of key tile `share(cta) + ahead` (valid where that
-// is below the work).  scratch: blockDim.x / 32 + 1 words of 64 bits and an AttnPos in shared memory.
 struct AttnScratch {
     int64_t warp[33];
+    int64_t at;     // place of the found sequence's first unit
+    int b;          // the sequence that holds the place looked for
     AttnPos pos;
 };
 
-__device__ __forceinline__ int64_t block_scan(int64_t x, AttnScratch *sc, int64_t *total) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    int64_t y = x;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
-        if (lane >= o) y += z;
+// Places of one head of a sequence; the lanes of a warp that called with `many` set get theirs from the
+// whole warp, one after the other.
+template <int ROWS, int KEYS, int COST>
+__device__ __forceinline__ int64_t attn_head_work(const AttnSeq<ROWS, KEYS> &q, bool live) {
+    int64_t w = 0;
+    const bool many = live && q.causal && q.tiles > 2;
+    if (live && !many) {
+        w = q.tiles ? int64_t(q.tiles) * (q.key_tiles(0) + COST) : 0;
+        if (q.causal && q.tiles == 2) w += q.key_tiles(1) - q.key_tiles(0);
     }
-    __syncthreads();
-    if (lane == 31) sc->warp[w] = y;
-    __syncthreads();
-    int64_t before = 0, all = 0;
-    for (int i = 0; i < nw; ++i) {
-        const int64_t v = sc->warp[i];
-        if (i < w) before += v;
-        all += v;
-    }
-    *total = all;
-    return before + y - x;  // exclusive
-}
-
-template <int ROWS, int KEYS, typename PickTile>
-__device__ __forceinline__ int64_t attn_locate(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io,
-                                               AttnScratch *sc, PickTile pick, bool report) {
-    // pass 1: the total (and, for batches of one chunk, each sequence's work in a register)
-    int64_t work = 0, mine = 0;
-    for (int b0 = 0; b0 < bt.batch; b0 += blockDim.x) {
-        const int b = b0 + threadIdx.x;
-        mine = 0;
-        if (b < bt.batch) {
-            const KvSeq s = load_seq(bt, c, b);
-            if (s.bad && report) flag_bad_page();
-            if (s.q1 > s.q0) mine = AttnSeq<ROWS, KEYS>(s, io).head_work() * c.kv_heads;
-        }
-        int64_t t;
-        block_scan(mine, sc, &t);
-        work += t;
-    }
-    if (threadIdx.x == 0) sc->pos.b = -1;
-    const int64_t want = work ? pick(work) : 0;  // uniform
-    int64_t before = 0;
-    for (int b0 = 0; b0 < bt.batch && work; b0 += blockDim.x) {
-        const int b = b0 + threadIdx.x;
-        if (bt.batch > blockDim.x) {
-            mine = 0;
-            if (b < bt.batch) {
-                const KvSeq s = load_seq(bt, c, b);
-                if (s.q1 > s.q0) mine = AttnSeq<ROWS, KEYS>(s, io).head_work() * c.kv_heads;
+    for (uint32_t rest = __ballot_sync(0xffffffffu, many); rest; rest &= rest - 1) {
+        const int src = __ffs(rest) - 1, lane = threadIdx.x & 31;
+        AttnSeq<ROWS, KEYS> x = q;
+        x.n = __shfl_sync(0xffffffffu, q.n, src);
+        x.s.kv = __shfl_sync(0xffffffffu, q.s.kv, src);
+        x.tiles = __shfl_sync(0xffffffffu, q.tiles, src);
+        int sum = 0;  // of at most 2^31 / ROWS tiles of 2^31 / KEYS keys: split where it could overflow
+        int64_t all = 0;
+        for (int mt = lane; mt < x.tiles; mt += 32) {
+            sum += x.key_tiles(mt);
+            if (sum > (1 << 29)) {
+                all += sum;
+                sum = 0;
             }
         }
-        int64_t t;
-        const int64_t at = before + block_scan(mine, sc, &t);
-        if (mine && at <= want && want < at + mine) {
-            const AttnSeq<ROWS, KEYS> q(load_seq(bt, c, b), io);
-            const int64_t per = mine / c.kv_heads, head = (want - at) / per;
-            int64_t rest = want - at - head * per;
-            int mt = 0;
-            while (rest >= q.key_tiles(mt)) rest -= q.key_tiles(mt++);
-            sc->pos = AttnPos{b, int(head), mt, int(rest), want - rest};
+        all += sum;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        if (lane == src) w = all + int64_t(x.tiles) * COST;
+    }
+    return w;
+}
+
+// All threads: the total work; sc->pos becomes the unit that holds place pick(shares), for which its
+// first key tile may lie before or behind that place.
+template <int ROWS, int KEYS, int COST, typename Pick>
+__device__ __forceinline__ int64_t attn_locate(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io,
+                                               AttnScratch *sc, Pick pick, bool report) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    int64_t work = 0, want = -1;
+    // one pass where the batch fits the block; else one for the total and one to find the place
+    const bool once = bt.batch <= int(blockDim.x);
+    for (int pass = once ? 1 : 0; pass < 2; ++pass) {
+        int64_t before = 0;
+        for (int b0 = 0; b0 < bt.batch; b0 += blockDim.x) {
+            const int b = b0 + threadIdx.x;
+            KvSeq s{0, 0, 0, false};
+            if (b < bt.batch) {
+                s = load_seq(bt, c, b);
+                if (s.bad && report && pass == 1) flag_bad_page();
+            }
+            const AttnSeq<ROWS, KEYS> q(s, io);
+            const int64_t head = attn_head_work<ROWS, KEYS, COST>(q, q.n > 0);
+            const int64_t mine = head * c.kv_heads;
+            int64_t y = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
+                if (lane >= o) y += z;
+            }
+            __syncthreads();
+            if (lane == 31) sc->warp[w] = y;
+            __syncthreads();
+            int64_t all = 0;
+            int64_t at = before + y - mine;
+            for (int i = 0; i < nw; ++i) {
+                const int64_t v = sc->warp[i];
+                if (i < w) at += v;
+                all += v;
+            }
+            before += all;
+            if (once) {
+                work = all;
+                want = work ? pick(AttnShares(work, gridDim.x)) : -1;
+            }
+            if (pass == 1 && mine && at <= want && want < at + mine) {
+                sc->b = b;
+                sc->at = at;
+                sc->warp[32] = head;
+            }
         }
-        before += t;
+        if (pass == 0) {
+            work = before;
+            want = work ? pick(AttnShares(work, gridDim.x)) : -1;
+        }
+    }
+    __syncthreads();
+    if (work == 0) return 0;
+    if (w == 0) {
+        // the unit within the sequence: every lane of warp 0 takes a row tile of the head
+        const int b = sc->b;
+        const AttnSeq<ROWS, KEYS> q(load_seq(bt, c, b), io);
+        const int64_t per = sc->warp[32], head = div64(want - sc->at, per);
+        int64_t unit = sc->at + head * per;  // place of the unit of row tile m0
+        const int64_t rest = want - unit;
+        AttnPos p{b, int(head), 0, 0};
+        if (!q.causal || q.tiles == 1) {
+            const int one = q.key_tiles(0) + COST;
+            p.mt = int(rest / one);
+            p.unit0 = unit + int64_t(p.mt) * one + COST;
+        } else {
+            for (int m0 = 0;; m0 += 32) {
+                const int n = m0 + lane < q.tiles ? q.key_tiles(m0 + lane) + COST : 0;
+                int64_t y = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int64_t z = __shfl_up_sync(0xffffffffu, y, o);
+                    if (lane >= o) y += z;
+                }
+                const uint32_t hit = __ballot_sync(0xffffffffu, unit + y > want);
+                if (hit || m0 + 32 >= q.tiles) {
+                    const int l = hit ? __ffs(hit) - 1 : 31;
+                    p.mt = m0 + l;
+                    p.unit0 = unit + __shfl_sync(0xffffffffu, y - n, l) + COST;
+                    break;
+                }
+                unit += __shfl_sync(0xffffffffu, y, 31);
+            }
+        }
+        if (lane == 0) sc->pos = p;
     }
     __syncthreads();
     return work;
 }
 
-// The unit behind p's (p is moved to its first key tile); b reaches bt.batch behind the last.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ void attn_next(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io,
-                                          AttnPos &p, const AttnSeq<ROWS, KEYS> &q) {
-    p.unit0 += q.key_tiles(p.mt);
-    p.tile = 0;
+// The unit behind p's; b reaches bt.batch behind the last.
+template <int ROWS, int KEYS, int COST>
+__device__ __forceinline__ void attn_next(const KvCacheView &c, const KvBatchView &bt, AttnPos &p,
+                                          const AttnSeq<ROWS, KEYS> &q) {
+    p.unit0 += q.key_tiles(p.mt) + COST;
     if (++p.mt < q.tiles) return;
     p.mt = 0;
     if (++p.head < c.kv_heads) return;
@@ -174,6 +242,36 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two fp32 operations at once
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 // The exponent of 2 that the row of a bf16 query is multiplied by so that it fits fp16 (its
@@ -235,68 +333,96 @@ __device__ __forceinline__ uint32_t h2fma(uint32_t a, uint32_t b, uint32_t c) {
 __device__ __forceinline__ uint32_t dup16(uint32_t x) { return __byte_perm(x, x, 0x1010); }
 
 // Joins the partial results of the unit that CTA `blockIdx.x` of the attention kernel began and did
-// not finish, every gridDim.y-th four rows of it: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.
-template <int ROWS, int KEYS, int D>
-__global__ void __launch_bounds__(128) attn_join_kernel(KvCacheView c, KvBatchView bt, AttnIO io) {
+// not finish: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.  A row's parts are shared by 1, 2, 4 or 8 of the
+// eight warps, at most 8 parts a warp where there are that many; the order of the sums is fixed by the parts.
+constexpr int kJoinWarps = 8;
+template <int ROWS, int KEYS, int COST, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(KvCacheView c, KvBatchView bt, AttnIO io) {
     __shared__ AttnScratch sc;
+    __shared__ __align__(16) float so[kJoinWarps][D];
+    __shared__ float sl[kJoinWarps];
     const int cta = blockIdx.x;
-    const int64_t work = attn_locate<ROWS, KEYS>(
-        c, bt, io, &sc,
-        [&](int64_t w) {
-            const int n = attn_ctas(w, gridDim.x);
-            return attn_share(w, min(cta + 1, n), n) - 1;  // the share's last key tile
-        },
+    const int64_t work = attn_locate<ROWS, KEYS, COST>(
+        c, bt, io, &sc, [&](const AttnShares &s) { return s.begin(min(cta + 1, s.ctas)) - 1; },  // the share's last place
         false);
     pdl_wait();  // the partial results are the kernel before's; waited for by every CTA
-    const int ctas = attn_ctas(work, gridDim.x);
-    if (cta >= ctas) return;
+    const AttnShares shares(work, gridDim.x);
+    if (cta >= shares.ctas) return;
     const AttnPos p = sc.pos;
-    const int64_t lo = attn_share(work, cta, ctas), hi = attn_share(work, cta + 1, ctas);
-    if (p.unit0 < lo) return;  // begun elsewhere
+    const int64_t lo = shares.begin(cta), hi = shares.begin(cta + 1);
+    if (p.unit0 < lo || p.unit0 >= hi) return;  // begun elsewhere
     const AttnSeq<ROWS, KEYS> q(load_seq(bt, c, p.b), io);
     const int64_t end = p.unit0 + q.key_tiles(p.mt);
     if (end <= hi) return;  // finished where it was begun
-    const int last = attn_owner(work, end - 1, ctas);
-    const int lane = threadIdx.x & 31;
+    const int np = shares.owner(end - 1) - cta + 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int share = np > 32 ? 8 : np > 16 ? 4 : np > 8 ? 2 : 1;  // warps of a row
+    const int sub = warp % share, rows = kJoinWarps / share;        // rows at once
+    const int nrows = int(min(unsigned(ROWS), unsigned(q.n) * unsigned(q.group) - unsigned(p.mt) * ROWS));
     using P = AttnPart<ROWS, D>;
-    for (int row = blockIdx.y * 4 + (threadIdx.x >> 5); row < ROWS; row += 4 * gridDim.y) {
-        const int64_t r = int64_t(p.mt) * ROWS + row;
-        if (r >= int64_t(q.n) * q.group) return;
-        float m = -INFINITY;
-        for (int i = cta + lane; i <= last; i += 32) m = fmaxf(m, P::slot(io.part, i, i == cta)[ROWS * D + row]);
-        m = warp_max(m);
-        const float base = m == -INFINITY ? 0.0f : m;
-        constexpr int V = D / 32;
+    constexpr int V = D / 32;
+    for (int r0 = blockIdx.y * rows; r0 < nrows; r0 += rows * gridDim.y) {
+        const int row = r0 + warp / share;
+        const bool live = row < nrows;
         float o[V] = {}, l = 0.0f;
-        for (int i = cta; i <= last; ++i) {
-            const float *s = P::slot(io.part, i, i == cta);
-            const float a = ex2(s[ROWS * D + row] - base);
-            l += a * s[ROWS * D + ROWS + row];
-            if constexpr (V == 2) {
-                const float2 x = *reinterpret_cast<const float2 *>(s + row * D + lane * 2);
-                o[0] += a * x.x;
-                o[1] += a * x.y;
-            } else {
-#pragma unroll
-                for (int j = 0; j < V / 4; ++j) {
-                    const float4 x = *reinterpret_cast<const float4 *>(s + row * D + j * 128 + lane * 4);
-                    o[4 * j] += a * x.x;
-                    o[4 * j + 1] += a * x.y;
-                    o[4 * j + 2] += a * x.z;
-                    o[4 * j + 3] += a * x.w;
+        if (live) {
+            float m = -INFINITY;
+            for (int i = lane; i < np; i += 32) m = fmaxf(m, P::slot(io.part, cta + i, i == 0)[ROWS * D + row]);
+            m = warp_max(m);
+            const float base = m == -INFINITY ? 0.0f : m;
+            for (int i0 = sub * 8; i0 < np; i0 += share * 8) {
+                // eight parts at a time: their weights on lanes 0..7, their loads in flight together
+                float a = 0.0f, pl = 0.0f;
+                if (lane < 8 && i0 + lane < np) {
+                    const float *s = P::slot(io.part, cta + i0 + lane, i0 + lane == 0) + ROWS * D + row;
+                    a = ex2(s[0] - base);
+                    pl = a * s[ROWS];
                 }
+                float x[8][V];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i0 + i < np) {
+                        const float *s = P::slot(io.part, cta + i0 + i, i0 + i == 0) + row * D + lane * V;
+#pragma unroll
+                        for (int j = 0; j < V; j += 2) {
+                            const float2 y = *reinterpret_cast<const float2 *>(s + j);
+                            x[i][j] = y.x;
+                            x[i][j + 1] = y.y;
+                        }
+                    }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i0 + i < np) {
+                        const float ai = __shfl_sync(0xffffffffu, a, i);
+                        l += __shfl_sync(0xffffffffu, pl, i);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) o[j] += ai * x[i][j];
+                    }
             }
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int token = q.s.q0 + int(r / q.group), h = p.head * q.group + int(r % q.group);
-        uint32_t *out = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(io.out) +
-                                                     (int64_t(token) * io.heads + h) * D);
+        if (share > 1) {  // uniform: the warps of a row meet
+            __syncthreads();
 #pragma unroll
-        for (int j = 0; j < V / 2; ++j) {
-            const int at = V == 2 ? lane : (j / 2) * 64 + lane * 2 + (j & 1);
-            out[at] = io.q_bf16 ? pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv)
-                                : pack_half(o[2 * j] * inv, o[2 * j + 1] * inv);
+            for (int j = 0; j < V; ++j) so[warp][lane * V + j] = o[j];
+            if (lane == 0) sl[warp] = l;
+            __syncthreads();
+            if (sub == 0)
+                for (int i = 1; i < share; ++i) {
+                    l += sl[warp + i];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) o[j] += so[warp + i][lane * V + j];
+                }
         }
+        if (!live || sub) continue;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const unsigned r = unsigned(p.mt) * ROWS + row;
+        const int token = q.s.q0 + int(r / unsigned(q.group)), h = p.head * q.group + int(r % unsigned(q.group));
+        uint32_t *out = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(io.out) +
+                                                     (int64_t(token) * io.heads + h) * D) + lane * (V / 2);
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j)
+            out[j] = io.q_bf16 ? pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv)
+                               : pack_half(o[2 * j] * inv, o[2 * j + 1] * inv);
     }
 }
 
@@ -305,19 +431,19 @@ struct AttnTiles {
     int rows, keys, occ;
 };
 
-template <int ROWS, int KEYS, int D>
+template <int ROWS, int KEYS, int COST, int D>
 static int attn_join_launch(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
                             cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas, std::min(ROWS / 4, 8));
-    cfg.blockDim = 128;
+    cfg.blockDim = kJoinWarps * 32;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_join_kernel<ROWS, KEYS, D>, c, bt, io);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_join_kernel<ROWS, KEYS, COST, D>, c, bt, io);
     return e == cudaSuccess ? ANVIL_OK : cuda_fail(e, "paged_attention join launch");
 }
 

@@ -32,6 +32,7 @@ namespace anvil {
 constexpr int kRowsWarps = 4;
 constexpr int kRowsStep = 16;   // keys of a warp's step
 constexpr int kRowsKeys = 64;   // keys of a key tile: one step of each warp
+constexpr int kRowsCost = 0;    // beginning and ending a unit, in key tiles
 
 template <int KIND, int D, int NT> struct RowsShape {
     static constexpr int rows = 8 * NT;                     // query rows of a unit
@@ -135,17 +136,12 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
     uint8_t *ring = smem + warp * S::per_warp;
     const bool whole = c.page_shift >= 4;
 
-    const int64_t work = attn_locate<ROWS, kRowsKeys>(
-        c, bt, io, &sc,
-        [&](int64_t w) {
-            const int n = attn_ctas(w, gridDim.x);
-            return attn_share(w, min(int(blockIdx.x), n - 1), n);
-        },
-        blockIdx.x == 0);
+    const int64_t work = attn_locate<ROWS, kRowsKeys, kRowsCost>(
+        c, bt, io, &sc, [&](const AttnShares &s) { return s.begin(min(int(blockIdx.x), s.ctas - 1)); }, blockIdx.x == 0);
     pdl_launch_dependents();
-    const int ctas = attn_ctas(work, gridDim.x);
-    if (int(blockIdx.x) >= ctas) return;
-    const int64_t lo = attn_share(work, blockIdx.x, ctas), hi = attn_share(work, blockIdx.x + 1, ctas);
+    const AttnShares shares(work, gridDim.x);
+    if (int(blockIdx.x) >= shares.ctas) return;
+    const int64_t lo = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
     AttnPos p = sc.pos;
     int slot = 0, fill = 0;     // ring slots: next to be worked on, next to be filled
 
@@ -154,7 +150,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
         const int ntiles = q.key_tiles(p.mt), nkeys = q.keys(p.mt);
         const int t0 = int(max(lo - p.unit0, int64_t(0))), t1 = int(min(hi - p.unit0, int64_t(ntiles)));
         const int key_end = min(t1 * kRowsKeys, nkeys);
-        const int nrows = int(min(int64_t(ROWS), int64_t(q.n) * q.group - int64_t(p.mt) * ROWS));
+        const int nrows = int(min(int64_t(ROWS), int64_t(unsigned(q.n) * unsigned(q.group) - unsigned(p.mt) * ROWS)));
 
         // ---- the ring: step s covers keys 16 s .. 16 s + 15
         const int step0 = t0 * 4 + warp, steps = (key_end + kRowsStep - 1) / kRowsStep;
@@ -233,8 +229,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int r = 8 * t + g;
-            const int64_t rr = int64_t(p.mt) * ROWS + r;
-            const int tok = int(rr / q.group), h = p.head * q.group + int(rr - int64_t(tok) * q.group);
+            const unsigned rr = unsigned(p.mt) * ROWS + r;
+            const int tok = int(rr / unsigned(q.group)), h = p.head * q.group + int(rr - unsigned(tok) * q.group);
             const bool live = r < nrows;
             const int my_seen = live ? kv_seen(tok, q.n, q.s.kv, q.causal) : 0;
             const uint16_t *src = static_cast<const uint16_t *>(io.q) + (q.s.q0 + int64_t(tok)) * io.q_row + h * io.q_head;
@@ -279,7 +275,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
             }
         }
         // every row of the unit sees the keys below this: no mask is needed there
-        const int free_end = min(key_end, kv_seen(int(int64_t(p.mt) * ROWS / q.group), q.n, q.s.kv, q.causal));
+        const int free_end = min(key_end, kv_seen(int(unsigned(p.mt) * ROWS / unsigned(q.group)), q.n, q.s.kv, q.causal));
 
         float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -597,8 +593,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                 sum += mw[w] * reinterpret_cast<float *>(smem + w * S::per_warp)[ROWS * (D + 4) + ROWS + r];
             }
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const int64_t rr = int64_t(p.mt) * ROWS + r;
-            const int tok = int(rr / q.group), h = p.head * q.group + int(rr - int64_t(tok) * q.group);
+            const unsigned rr = unsigned(p.mt) * ROWS + r;
+            const int tok = int(rr / unsigned(q.group)), h = p.head * q.group + int(rr - unsigned(tok) * q.group);
             uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(io.out) +
                                                          ((int64_t(q.s.q0) + tok) * io.heads + h) * D);
 #pragma unroll
@@ -622,7 +618,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
             }
         }
         __syncthreads();  // before the rings are filled again
-        attn_next(c, bt, io, p, q);
+        attn_next<ROWS, kRowsKeys, kRowsCost>(c, bt, p, q);
     }
 }
 
@@ -642,7 +638,7 @@ template <int KIND, int D, int NT> struct RowsOps {
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
         attn_rows_kernel<KIND, D, NT><<<ctas, kRowsWarps * 32, S::smem, stream>>>(c, bt, io);
         if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "paged_attention launch");
-        return join ? attn_join_launch<S::rows, kRowsKeys, D>(c, bt, io, ctas, stream) : ANVIL_OK;
+        return join ? attn_join_launch<S::rows, kRowsKeys, kRowsCost, D>(c, bt, io, ctas, stream) : ANVIL_OK;
     }
 };
 

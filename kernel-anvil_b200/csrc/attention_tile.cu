@@ -23,6 +23,7 @@
 namespace anvil {
 
 constexpr int kTileThreads = 512;
+constexpr int kTileCost = 4;        // beginning and ending a unit, in key tiles
 constexpr float kTileSlack = 8.0f;  // log2 of how far weights may exceed 1
 
 template <int KIND, int D> struct TileShape {
@@ -98,10 +99,25 @@ struct TileShared {
     int64_t row[2][128];    // loader: cache rows of a key tile, by parity
 };
 
+// try_wait that may sleep for up to 20 us: 13 warps that poll take issue slots from the softmax
+__device__ __forceinline__ bool mbar_try_wait_long(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000)
+        : "memory");
+    return ok != 0;
+}
+
 __device__ __forceinline__ void tile_wait(TileShared *sh, uint64_t *bar, uint32_t parity, uint64_t limit_ns) {
-    if (mbar_try_wait(bar, parity)) return;
+    if (mbar_try_wait_long(bar, parity)) return;
     const uint64_t t0 = global_timer_ns();
-    while (!mbar_try_wait(bar, parity)) {
+    while (!mbar_try_wait_long(bar, parity)) {
         if (*reinterpret_cast<volatile int *>(&sh->failed)) return;
         if (global_timer_ns() - t0 > limit_ns) {
             *reinterpret_cast<volatile int *>(&sh->failed) = 1;
@@ -125,9 +141,9 @@ template <int KIND, int D> struct TileUnit {
         t0 = int(max(lo - p.unit0, int64_t(0)));
         t1 = int(min(hi - p.unit0, int64_t(ntiles)));
         key_end = min(t1 * S::keys, q.keys(p.mt));
-        nrows = int(min(int64_t(S::rows), int64_t(q.n) * q.group - int64_t(p.mt) * S::rows));
+        nrows = int(min(int64_t(S::rows), int64_t(unsigned(q.n) * unsigned(q.group) - unsigned(p.mt) * S::rows)));
         // every row of the unit sees the keys below this
-        free_end = min(key_end, kv_seen(int(int64_t(p.mt) * S::rows / q.group), q.n, q.s.kv, q.causal));
+        free_end = min(key_end, kv_seen(int(unsigned(p.mt) * S::rows / unsigned(q.group)), q.n, q.s.kv, q.causal));
     }
 };
 
@@ -142,17 +158,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     uint8_t *sq = base, *sbuf = base + S::q_bytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    const int64_t work = attn_locate<S::rows, S::keys>(
-        c, bt, io, &sh.sc,
-        [&](int64_t w) {
-            const int n = attn_ctas(w, gridDim.x);
-            return attn_share(w, min(int(blockIdx.x), n - 1), n);
-        },
-        blockIdx.x == 0);
+    const int64_t work = attn_locate<S::rows, S::keys, kTileCost>(
+        c, bt, io, &sh.sc, [&](const AttnShares &s) { return s.begin(min(int(blockIdx.x), s.ctas - 1)); }, blockIdx.x == 0);
     pdl_launch_dependents();
-    const int ctas = attn_ctas(work, gridDim.x);
-    if (int(blockIdx.x) >= ctas) return;
-    const int64_t lo = attn_share(work, blockIdx.x, ctas), hi = attn_share(work, blockIdx.x + 1, ctas);
+    const AttnShares shares(work, gridDim.x);
+    if (int(blockIdx.x) >= shares.ctas) return;
+    const int64_t lo = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
     AttnPos p = sh.sc.pos;
 
     if (threadIdx.x == 0) {
@@ -195,8 +206,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     // ---- this row's query, into the swizzled operand
                     const int ur = w * 128 + r;
                     const bool live = ur < u.nrows;
-                    const int64_t rr = int64_t(p.mt) * S::rows + ur;
-                    const int tok = int(rr / u.q.group), h = p.head * u.q.group + int(rr - int64_t(tok) * u.q.group);
+                    const unsigned rr = unsigned(p.mt) * S::rows + ur;
+                    const int tok = int(rr / unsigned(u.q.group)), h = p.head * u.q.group + int(rr - unsigned(tok) * u.q.group);
                     const int seen = live ? min(u.key_end, kv_seen(tok, u.q.n, u.q.s.kv, u.q.causal)) : 0;
                     const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(io.q) +
                                                                        (u.q.s.q0 + int64_t(tok)) * io.q_row + h * io.q_head);
@@ -270,7 +281,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                 mask(s + 32, i + 1);
                             }
 #pragma unroll
-                            for (int j = 0; j < 64; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(s[j]));
+                            for (int j = 0; j < 64; j += 2)
+                                mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
                         }
                         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                         const float mt = top * fac;
@@ -297,7 +309,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             m = mn;
                         }
                         const float nb = m == -INFINITY ? 0.0f : -m;
-                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        const uint64_t fac2 = pack2(fac, fac), nb2 = pack2(nb, nb);
+                        uint64_t sum[2] = {0, 0};
                         uint32_t s[2][32];
                         tmem_ld32(ts, s[0]);
 #pragma unroll
@@ -309,16 +322,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             uint32_t y[16];
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
-                                const float e0 = ex2(fmaf(__uint_as_float(x[2 * j]), fac, nb));
-                                const float e1 = ex2(fmaf(__uint_as_float(x[2 * j + 1]), fac, nb));
-                                sum[j & 1] += e0;
-                                sum[2 + (j & 1)] += e1;
+                                float e0, e1;
+                                unpack2(fma2(pack2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), fac2, nb2), e0, e1);
+                                e0 = ex2(e0);
+                                e1 = ex2(e1);
+                                sum[j & 1] = add2(sum[j & 1], pack2(e0, e1));
                                 y[j] = BF ? pack_bf16(e0, e1) : pack_half(e0, e1);
                             }
                             tmem_st16(ts + 16 * i, y);  // over scores already read
                         }
-                        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                        {
+                            float a0, a1;
+                            unpack2(add2(sum[0], sum[1]), a0, a1);
+                            l += a0 + a1;
+                        }
                         wait_st();
+                        // A wait on a parity holds only while the phase before is known to be over.  Where scores run
+                        // ahead of the last tile's P V (one row tile) nothing else has shown that yet.
+                        if (S::nq == 1 && !first) tile_wait(&sh, &sh.pv_done[w], (npv - 1) & 1, limit_ns);
                         fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&sh.p_full[w]);
@@ -381,7 +402,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     fence_before();
                 }
                 seq += u.t1 - u.t0;
-                attn_next(c, bt, io, p, u.q);
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
             }
     } else if (warp < 12) {
         // ================= loader: 128 threads, keys then values of each tile ========================
@@ -514,7 +535,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 }
             }
-            attn_next(c, bt, io, p, u.q);
+            attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
         }
         if (!S::quant && pending >= 0) {
             asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -584,7 +605,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     if (S::nq == 2 && more) mma_commit(&sh.empty[bk % S::nbuf]);
                 }
                 nb += 2 * tiles;
-                attn_next(c, bt, io, p, u.q);
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
             }
             mma_commit(&sh.drain);
             tile_wait(&sh, &sh.drain, 0, limit_ns);
@@ -606,7 +627,7 @@ template <int KIND, int D> static int launch_tile(const KvCacheView &c, const Kv
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
     attn_tile_kernel<KIND, D><<<ctas, kTileThreads, S::smem, stream>>>(c, bt, io, wait_limit_ns());
     if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "paged_attention launch");
-    return join ? attn_join_launch<S::rows, S::keys, D>(c, bt, io, ctas, stream) : ANVIL_OK;
+    return join ? attn_join_launch<S::rows, S::keys, kTileCost, D>(c, bt, io, ctas, stream) : ANVIL_OK;
 }
 
 template <int KIND> static int tile_dim(int D, const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
