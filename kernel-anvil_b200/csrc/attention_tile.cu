@@ -2,12 +2,15 @@
 // the fifth-generation tensor cores.
 //
 // A CTA, one per SM, works on a unit of 256 query rows (two tiles of 128; one tile where head_dim is
-// 256) against tiles of 128 keys (64), with S and O in tensor memory:
+// 256) against tiles of 64 keys, with S and O in tensor memory:
 //   S = Q K^T          tcgen05.mma, both operands in shared memory
 //   P = 2^(S f - m)    one thread a row: no shuffles; P goes back over S in 16 bits
 //   O += P V           tcgen05.mma with P from tensor memory, V transposed by its descriptor
-// Warp roles: warps 0-3 and 4-7 are the softmax of the two row tiles, which alternate so that one
-// tile's exponentials run under the other's products; warps 8-11 bring keys and values through
+// S has two turns of 64 columns a row tile, so the scores of the next keys are there when the weights of
+// the last ones are done, and the softmax never waits for a product that waits for it.  (Tiles of 128
+// keys fill tensor memory with one turn, P over S: the chain softmax, P V, Q K^T, softmax then left
+// both sides idle half of the time: 2.68 against FILLCHUNK ms for 2048 rows over 30049 keys.)
+// Warp roles: warps 0-3 and 4-7 are the softmax of the two row tiles; warps 8-11 bring keys and values through
 // the page table into a ring of buffers in the 128-byte swizzled layout, widening quantised codes
 // to fp16 on the way; warp 12 issues every product.  All hand-over is by mbarriers; each wait is
 // bounded and a failure makes the later ones return at once.
@@ -23,30 +26,34 @@
 namespace anvil {
 
 constexpr int kTileThreads = 512;
-constexpr int kTileCost = 4;        // beginning and ending a unit, in key tiles
+constexpr int kTileCost = 8;        // beginning and ending a unit, in key tiles
 constexpr float kTileSlack = 8.0f;  // log2 of how far weights may exceed 1
 
 template <int KIND, int D> struct TileShape {
     static constexpr int nq = D == 256 ? 1 : 2;         // row tiles of 128
     static constexpr int rows = 128 * nq;
-    static constexpr int keys = D == 256 ? 64 : 128;
+    static constexpr int keys = 64;
     static constexpr int blocks = D / 64;               // 64-value column blocks of an operand
     static constexpr int q_bytes = rows * D * 2;
     static constexpr int buf = keys * D * 2;            // one buffer: keys or values of a tile
-    static constexpr int nbuf = D == 64 ? 6 : 4;
+    static constexpr int nbuf = D == 256 ? 4 : 8;
     static constexpr int smem = 1024 + q_bytes + nbuf * buf;
     static constexpr bool bf16 = KIND == kKvBF16;
     static constexpr bool quant = KIND == kKvQ8_0 || KIND == kKvQ4_0;
-    // tensor memory columns: S of the two tiles (or two turns of one), then O
-    static constexpr int s_cols = keys, o_col = 2 * keys, o_cols = D;
+    // tensor memory columns: two turns of S for each row tile, then O
+    static constexpr int s_cols = keys, o_col = 4 * keys, o_cols = D;
 };
 
 // ---- tcgen05 ----------------------------------------------------------------------------------
 
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    // start, leading and stride byte offsets in 16-byte units; version 1; 128-byte swizzle
-    return uint64_t((addr & 0x3FFFF) >> 4) | (uint64_t(lbo >> 4) << 16) | (uint64_t(sbo >> 4) << 32) |
-           (uint64_t(1) << 46) | (uint64_t(2) << 61);
+// A shared-memory operand in the 128-byte swizzle: low word start and leading byte offset, high word stride
+// byte offset 1024 (eight rows), version 1 and the swizzle; offsets in 16-byte units.
+__device__ __forceinline__ uint32_t smem_desc_lo(uint32_t addr, uint32_t lbo) {
+    return ((addr & 0x3FFFF) >> 4) | ((lbo >> 4) << 16);
+}
+__device__ __forceinline__ uint64_t smem_desc(uint32_t lo) {
+    constexpr uint32_t hi = (1024 >> 4) | (1u << 14) | (2u << 29);
+    return uint64_t(lo) | (uint64_t(hi) << 32);
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
@@ -65,6 +72,14 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One lane of the warp.  (Code under this predicate keeps the operands of the instructions below in uniform
+// registers; under lane == 0 every one of them is moved there first: 85 cycles a product to issue.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t e;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(e));
+    return e != 0;
+}
 
 #define R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
 #define W8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
@@ -91,35 +106,25 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
 
 struct TileShared {
     AttnScratch sc;
-    uint64_t full[6], empty[6], q_full[2], s_full[2], p_full[2], pv_done[2], drain;
+    uint64_t full[8], empty[8], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], drain;  // [row tile][turn]
     uint32_t tmem;
     int failed;             // a wait gave up: later ones do not wait
     int dirty[8];           // [unit % 8] = unit where non-finite values were taken out of its value tiles
-    uint32_t bad[4][4];     // [tile % 4]: keys without a page
-    int64_t row[2][128];    // loader: cache rows of a key tile, by parity
+    uint32_t bad[8][2];     // [tile % 8]: keys without a page
+    int64_t row[2][64];    // loader: cache rows of a key tile, by parity
 };
 
-// try_wait that may sleep for up to 20 us: 13 warps that poll take issue slots from the softmax
-__device__ __forceinline__ bool mbar_try_wait_long(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(20000)
-        : "memory");
-    return ok != 0;
-}
-
+// Bounded by the wall clock, which is only looked at after some hundred polls: reading it takes longer
+// than most waits.
 __device__ __forceinline__ void tile_wait(TileShared *sh, uint64_t *bar, uint32_t parity, uint64_t limit_ns) {
-    if (mbar_try_wait_long(bar, parity)) return;
-    const uint64_t t0 = global_timer_ns();
-    while (!mbar_try_wait_long(bar, parity)) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {
+        if (i & 255) continue;
         if (*reinterpret_cast<volatile int *>(&sh->failed)) return;
-        if (global_timer_ns() - t0 > limit_ns) {
+        const uint64_t now = global_timer_ns();
+        if (t0 == 0) {
+            t0 = now;
+        } else if (now - t0 > limit_ns) {
             *reinterpret_cast<volatile int *>(&sh->failed) = 1;
             atomicOr(&g_anvil_device_status, kStatusMbarTimeout);
             return;
@@ -173,9 +178,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.q_full[i], 4);
-            mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.p_full[i], 4);
-            mbar_init(&sh.pv_done[i], 1);
+            for (int x = 0; x < 2; ++x) {
+                mbar_init(&sh.s_full[i][x], 1);
+                mbar_init(&sh.p_full[i][x], 4);
+                mbar_init(&sh.pv_done[i][x], 1);
+            }
         }
         mbar_init(&sh.drain, 1);
         mbar_fence_init();
@@ -196,7 +203,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
         const int w = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        uint32_t ns[2] = {0, 0}, npv = 0;   // completions waited for: S by buffer, PV of this tile
+        // Tiles so far on each turn.  S, P and P V of a tile use its turn's barriers: a side may be a whole tile
+        // ahead of the other, and a parity tells one phase from the next only.
+        uint32_t n0 = 0, n1 = 0;
         int unit = 0, seq = 0;              // units and key tiles so far, counted alike in every role
         if (w < S::nq)
             while (p.b < bt.batch && p.unit0 < hi) {
@@ -250,49 +259,35 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     if (lane == 0) mbar_arrive(&sh.q_full[w]);
 
                     float m = -INFINITY, l = 0.0f;
+                    const uint32_t to = tmem + lanes + S::o_col + w * S::o_cols;
                     for (int t = u.t0; t < u.t1; ++t) {
-                        const int x = S::nq == 2 ? w : (t - u.t0) & 1;
-                        const uint32_t ts = tmem + lanes + x * S::s_cols, to = tmem + lanes + S::o_col + (S::nq == 2 ? w * S::o_cols : 0);
-                        tile_wait(&sh, &sh.s_full[x], ns[x]++ & 1, limit_ns);
+                        const int x = (t - u.t0) & 1;
+                        const uint32_t ts = tmem + lanes + (w * 2 + x) * S::s_cols;
+                        tile_wait(&sh, &sh.s_full[w][x], (x ? n1 : n0) & 1, limit_ns);
                         __syncwarp();
                         fence_after();
-                        const int key0 = t * S::keys;
-                        uint32_t any_bad = 0;
+                        uint32_t s[64];
+                        tmem_ld32(ts, s);
+                        tmem_ld32(ts + 32, s + 32);
+                        const uint32_t bad[2] = {sh.bad[(seq + t - u.t0) & 7][0], sh.bad[(seq + t - u.t0) & 7][1]};
+                        wait_ld();
+                        if ((t + 1) * 64 > u.free_end || (bad[0] | bad[1])) {
+                            const int left = seen - t * 64;
 #pragma unroll
-                        for (int i = 0; i < S::keys / 32; ++i) any_bad |= sh.bad[(seq + t - u.t0) & 3][i];
-                        const bool masked = key0 + S::keys > u.free_end || any_bad;
-                        // 32 scores of this row; S is read twice rather than held in 128 registers
-                        auto mask = [&](uint32_t *s, int i) {
-                            const uint32_t bad = sh.bad[(seq + t - u.t0) & 3][i];
-                            const int left = seen - key0 - 32 * i;
-#pragma unroll
-                            for (int j = 0; j < 32; ++j)
-                                if (j >= left || ((bad >> j) & 1)) s[j] = 0xFF800000u;
-                        };
+                            for (int i = 0; i < 64; ++i)
+                                if (i >= left || ((bad[i >> 5] >> (i & 31)) & 1)) s[i] = 0xFF800000u;
+                        }
                         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int i = 0; i < S::keys / 32; i += 2) {
-                            uint32_t s[64];
-                            tmem_ld32(ts + 32 * i, s);
-                            tmem_ld32(ts + 32 * i + 32, s + 32);
-                            wait_ld();
-                            if (masked) {
-                                mask(s, i);
-                                mask(s + 32, i + 1);
-                            }
-#pragma unroll
-                            for (int j = 0; j < 64; j += 2)
-                                mx[(j >> 1) & 3] = max3(mx[(j >> 1) & 3], __uint_as_float(s[j]), __uint_as_float(s[j + 1]));
-                        }
-                        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                        const float mt = top * fac;
-                        const bool first = t == u.t0;
+                        for (int i = 0; i < 64; i += 2)
+                            mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac;
                         const bool raise = mt > m + kTileSlack || (m == -INFINITY && mt > m);
                         if (__any_sync(0xffffffffu, raise)) {
                             const float mn = raise ? mt : m;
                             const float a = raise ? ex2(m - mn) : 1.0f;
-                            if (!first) {
-                                tile_wait(&sh, &sh.pv_done[w], (npv - 1) & 1, limit_ns);
+                            if (t > u.t0) {
+                                tile_wait(&sh, &sh.pv_done[w][x ^ 1], ((x ? n0 : n1) - 1) & 1, limit_ns);  // the last tile's P V
                                 __syncwarp();
                                 fence_after();
 #pragma unroll 1
@@ -311,45 +306,31 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         const float nb = m == -INFINITY ? 0.0f : -m;
                         const uint64_t fac2 = pack2(fac, fac), nb2 = pack2(nb, nb);
                         uint64_t sum[2] = {0, 0};
-                        uint32_t s[2][32];
-                        tmem_ld32(ts, s[0]);
 #pragma unroll
-                        for (int i = 0; i < S::keys / 32; ++i) {
-                            uint32_t *x = s[i & 1];
-                            wait_ld();
-                            if (i + 1 < S::keys / 32) tmem_ld32(ts + 32 * (i + 1), s[(i + 1) & 1]);
-                            if (masked) mask(x, i);
-                            uint32_t y[16];
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                float e0, e1;
-                                unpack2(fma2(pack2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), fac2, nb2), e0, e1);
-                                e0 = ex2(e0);
-                                e1 = ex2(e1);
-                                sum[j & 1] = add2(sum[j & 1], pack2(e0, e1));
-                                y[j] = BF ? pack_bf16(e0, e1) : pack_half(e0, e1);
-                            }
-                            tmem_st16(ts + 16 * i, y);  // over scores already read
+                        for (int i = 0; i < 32; ++i) {
+                            float e0, e1;
+                            unpack2(fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), fac2, nb2), e0, e1);
+                            e0 = ex2(e0);
+                            e1 = ex2(e1);
+                            sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
+                            s[i] = BF ? pack_bf16(e0, e1) : pack_half(e0, e1);
                         }
-                        {
-                            float a0, a1;
-                            unpack2(add2(sum[0], sum[1]), a0, a1);
-                            l += a0 + a1;
-                        }
+                        tmem_st32(ts, s);
+                        float a0, a1;
+                        unpack2(add2(sum[0], sum[1]), a0, a1);
+                        l += a0 + a1;
                         wait_st();
-                        // A wait on a parity holds only while the phase before is known to be over.  Where scores run
-                        // ahead of the last tile's P V (one row tile) nothing else has shown that yet.
-                        if (S::nq == 1 && !first) tile_wait(&sh, &sh.pv_done[w], (npv - 1) & 1, limit_ns);
                         fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.p_full[w]);
-                        ++npv;
+                        if (lane == 0) mbar_arrive(&sh.p_full[w][x]);
+                        (x ? n1 : n0) += 1;
                     }
 
                     // ---- the unit's outputs, or this share's part of them
-                    tile_wait(&sh, &sh.pv_done[w], (npv - 1) & 1, limit_ns);
+                    const int xl = (u.t1 - 1 - u.t0) & 1;  // the last tile's turn; its P V ends after all others
+                    tile_wait(&sh, &sh.pv_done[w][xl], ((xl ? n1 : n0) - 1) & 1, limit_ns);
+                    __syncwarp();
                     fence_after();
-                    const uint32_t to = tmem + lanes + S::o_col + (S::nq == 2 ? w * S::o_cols : 0);
                     const bool begun = p.unit0 < lo, unfinished = p.unit0 + u.ntiles > hi;
                     const bool dirty = *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) == unit;
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -409,48 +390,60 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         const int tid = threadIdx.x - 256;
         uint32_t nb = 0;        // buffers filled
-        int pending = -1;       // buffer whose copies were not announced yet
         int unit = 0, seq = 0;
         auto announce = [&](int b) {
             fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.full[b]);
         };
-        while (p.b < bt.batch && p.unit0 < hi) {
-            const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
-            ++unit;
-            for (int t = u.t0; t < u.t1; ++t, ++seq) {
-                // rows of this tile's keys
-                const int key = t * S::keys + tid;
-                int64_t row = -2;
-                if (tid < S::keys && key < u.key_end) row = kv_lookup(bt, c, p.b, key, p.head);
-                if (tid < S::keys) sh.row[seq & 1][tid] = row;
-                const uint32_t bad = __ballot_sync(0xffffffffu, row == -1);
+        // cache rows of key tile t, key by key, for everyone; rows of the keys behind the last: -2
+        auto rows_of = [&](const TileUnit<KIND, D> &u, int t) -> int64_t {
+            const int key = t * S::keys + tid;
+            return tid < S::keys && key < u.key_end ? kv_lookup(bt, c, p.b, key, p.head) : -2;
+        };
+        auto share_rows = [&](int64_t row, int at) {
+            const uint32_t bad = __ballot_sync(0xffffffffu, row == -1);
+            if (tid < S::keys) {
+                sh.row[at & 1][tid] = row;
                 if (lane == 0) {
-                    sh.bad[seq & 3][tid >> 5] = bad;
+                    sh.bad[at & 7][tid >> 5] = bad;
                     if (bad) flag_bad_page();
                 }
-                loader_sync();
-                const bool check = t * S::keys + S::keys > u.free_end;
-                for (int kv = 0; kv < 2; ++kv, ++nb) {
-                    const int b = nb % S::nbuf;
-                    if (nb >= S::nbuf) {
-                        const uint32_t parity = (nb / S::nbuf - 1) & 1;
-                        // (a product may wait for the pending buffer before it frees this one)
-                        if (!S::quant && pending >= 0 && !__all_sync(0xffffffffu, mbar_try_wait(&sh.empty[b], parity))) {
-                            asm volatile("cp.async.wait_group 0;" ::: "memory");
-                            announce(pending);
-                            pending = -1;
+            }
+            loader_sync();
+        };
+        if constexpr (!S::quant) {
+            // 16-bit rows go straight to their places; up to `depth` buffers' copies are in flight, announced in order
+            constexpr int CH = D / 8, depth = S::nbuf / 2;
+            int pending = 0;
+            auto settle = [&](int left) {  // all copies are done: announce all but the newest `left`
+                for (; pending > left; --pending) announce((nb - pending) % S::nbuf);
+            };
+            while (p.b < bt.batch && p.unit0 < hi) {
+                const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                ++unit;
+                int64_t row = rows_of(u, u.t0);
+                for (int t = u.t0; t < u.t1; ++t, ++seq) {
+                    share_rows(row, seq);
+                    if (t + 1 < u.t1) row = rows_of(u, t + 1);
+                    const bool check = t * S::keys + S::keys > u.free_end;
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const int b = nb % S::nbuf;
+                        if (nb >= S::nbuf) {
+                            const uint32_t parity = (nb / S::nbuf - 1) & 1;
+                            // (a product may wait for a pending buffer before it frees this one)
+                            if (pending && !__all_sync(0xffffffffu, mbar_try_wait(&sh.empty[b], parity))) {
+                                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                                settle(0);
+                            }
+                            tile_wait(&sh, &sh.empty[b], parity, limit_ns);
+                            __syncwarp();
                         }
-                        tile_wait(&sh, &sh.empty[b], parity, limit_ns);
-                    }
-                    uint8_t *dst = sbuf + b * S::buf;
-                    const uint8_t *src = kv ? c.v : c.k;
-                    if constexpr (!S::quant) {
-                        constexpr int CH = D / 8;  // chunks of a row
-#pragma unroll 4
-                        for (int i = tid; i < S::keys * CH; i += 128) {
-                            const int r = i / CH, ch = i % CH;
+                        uint8_t *dst = sbuf + b * S::buf;
+                        const uint8_t *src = kv ? c.v : c.k;
+#pragma unroll
+                        for (int i = 0; i < S::keys * CH / 128; ++i) {
+                            const int r = tid / CH + i * (128 / CH), ch = tid % CH;
                             const int64_t rw = sh.row[seq & 1][r];
                             const uint32_t to = smem_u32(dst + (ch >> 3) * (S::keys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
                             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to),
@@ -458,113 +451,145 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                          : "memory");
                         }
                         asm volatile("cp.async.commit_group;" ::: "memory");
+                        ++nb;
+                        ++pending;
                         if (kv && check) {
                             // a masked tile's values: what is not finite leaves the product (see the outputs)
                             asm volatile("cp.async.wait_group 0;" ::: "memory");
-                            for (int i = tid; i < S::keys * CH; i += 128) {
-                                const int r = i / CH, ch = i % CH;
-                                uint32_t *w4 = reinterpret_cast<uint32_t *>(dst + (ch >> 3) * (S::keys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const uint32_t bits = nonfinite2<BF>(w4[j]);
-                                    if (bits) {
-                                        w4[j] &= ~bits;
-                                        *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
-                                    }
+                            for (int i = 0; i < S::keys * CH / 128; ++i) {
+                                const int r = tid / CH + i * (128 / CH), ch = tid % CH;
+                                uint4 *w4 = reinterpret_cast<uint4 *>(dst + (ch >> 3) * (S::keys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                                uint4 x = *w4;
+                                const uint32_t n[4] = {nonfinite2<BF>(x.x), nonfinite2<BF>(x.y), nonfinite2<BF>(x.z), nonfinite2<BF>(x.w)};
+                                if (n[0] | n[1] | n[2] | n[3]) {
+                                    *w4 = make_uint4(x.x & ~n[0], x.y & ~n[1], x.z & ~n[2], x.w & ~n[3]);
+                                    *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
                                 }
                             }
+                            __syncwarp();
+                            settle(0);
+                        } else if (pending == depth) {
+                            asm volatile("cp.async.wait_group %0;" ::"n"(depth - 1) : "memory");
+                            settle(depth - 1);
                         }
-                        if (pending >= 0) {
-                            asm volatile("cp.async.wait_group 1;" ::: "memory");
-                            announce(pending);
-                        }
-                        pending = b;
-                    } else {
-                        // 16 bytes of codes a turn: 16 (Q8_0) or 32 (Q4_0) values, two or four chunks
-                        constexpr int RB = KvRow<KIND, D>::bytes, CH = RB / 16, N = S::keys * CH / 128;
-                        constexpr int OUT = KIND == kKvQ8_0 ? 2 : 4, VALS = 8 * OUT;
-                        const __half *scales = kv ? c.vs : c.ks;
-                        // eight lanes store two rows of four chunks where rows have them: distinct banks
-                        const int in = tid % (2 * CH);
-                        const int ch = CH >= 8 ? (in & 3) | ((in >> 3) << 2) : tid % CH;
-                        const int r0 = CH >= 8 ? tid / (2 * CH) * 2 + ((in >> 2) & 1) : tid / CH;
-                        uint4 w[N];
-                        uint16_t d[N];
-#pragma unroll
-                        for (int i = 0; i < N; ++i) {
-                            const int64_t rw = sh.row[seq & 1][r0 + i * (128 / CH)];
-                            w[i] = make_uint4(0, 0, 0, 0);
-                            d[i] = 0;
-                            if (rw >= 0) {
-                                w[i] = __ldg(reinterpret_cast<const uint4 *>(src + rw * RB + ch * 16));
-                                d[i] = __ldg(reinterpret_cast<const unsigned short *>(scales) + rw * (D / 32) + ch * VALS / 32);
-                            }
-                        }
-#pragma unroll
-                        for (int i = 0; i < N; ++i) {
-                            const int r = r0 + i * (128 / CH);
-                            uint32_t d2 = d[i] | (uint32_t(d[i]) << 16);
-                            if (kv && check && nonfinite2<false>(d2)) {
-                                d2 = 0;
-                                *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
-                            }
-                            const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-                            uint32_t y[4 * OUT];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                if constexpr (KIND == kKvQ8_0) {
-                                    const uint32_t v = x[j] ^ 0x80808080u;
-                                    y[2 * j] = h2mul(h2sub(__byte_perm(v, 0x64646464u, 0x4140), 0x64806480u), d2);
-                                    y[2 * j + 1] = h2mul(h2sub(__byte_perm(v, 0x64646464u, 0x4342), 0x64806480u), d2);
-                                } else {
-                                    const uint32_t a = x[j] & 0x0F0F0F0Fu, e = (x[j] >> 4) & 0x0F0F0F0Fu;
-                                    y[2 * j] = h2mul(h2sub(__byte_perm(a, 0x64646464u, 0x4140), 0x64086408u), d2);
-                                    y[2 * j + 1] = h2mul(h2sub(__byte_perm(a, 0x64646464u, 0x4342), 0x64086408u), d2);
-                                    y[8 + 2 * j] = h2mul(h2sub(__byte_perm(e, 0x64646464u, 0x4140), 0x64086408u), d2);
-                                    y[8 + 2 * j + 1] = h2mul(h2sub(__byte_perm(e, 0x64646464u, 0x4342), 0x64086408u), d2);
-                                }
-                            }
-#pragma unroll
-                            for (int j = 0; j < OUT; ++j) {
-                                const int oc = ch * OUT + j;
-                                *reinterpret_cast<uint4 *>(dst + (oc >> 3) * (S::keys * 128) + r * 128 + (((oc & 7) ^ (r & 7)) << 4)) =
-                                    make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
-                            }
-                        }
-                        announce(b);
                     }
                 }
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
             }
-            attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
-        }
-        if (!S::quant && pending >= 0) {
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            announce(pending);
+            settle(0);
+        } else {
+            // 16 bytes of codes a turn: 16 (Q8_0) or 32 (Q4_0) values, two or four chunks of 16 bytes.  The next
+            // buffer's codes are in flight while this one's are widened.
+            constexpr int RB = KvRow<KIND, D>::bytes, CH = RB / 16, N = S::keys * CH / 128;
+            constexpr int OUT = KIND == kKvQ8_0 ? 2 : 4, VALS = 8 * OUT;
+            // eight lanes store two rows of four chunks where rows have them: distinct banks
+            const int in = tid % (2 * CH);
+            const int ch = CH >= 8 ? (in & 3) | ((in >> 3) << 2) : tid % CH;
+            const int r0 = CH >= 8 ? tid / (2 * CH) * 2 + ((in >> 2) & 1) : tid / CH;
+            struct Codes {
+                uint4 w[N];
+                uint32_t d[N];
+            };
+            auto fetch = [&](Codes &x, int at, int kv) {
+                const uint8_t *src = kv ? c.v : c.k;
+                const unsigned short *scales = reinterpret_cast<const unsigned short *>(kv ? c.vs : c.ks);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int64_t rw = sh.row[at & 1][r0 + i * (128 / CH)];
+                    x.w[i] = make_uint4(0, 0, 0, 0);
+                    x.d[i] = 0;
+                    if (rw >= 0) {
+                        x.w[i] = __ldg(reinterpret_cast<const uint4 *>(src + rw * RB + ch * 16));
+                        x.d[i] = __ldg(scales + rw * (D / 32) + ch * VALS / 32);
+                    }
+                }
+            };
+            auto widen = [&](const Codes &x, bool check) {
+                const int b = nb % S::nbuf;
+                if (nb >= S::nbuf) tile_wait(&sh, &sh.empty[b], (nb / S::nbuf - 1) & 1, limit_ns);
+                __syncwarp();
+                uint8_t *dst = sbuf + b * S::buf;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int r = r0 + i * (128 / CH);
+                    uint32_t d2 = dup16(x.d[i]);
+                    if (check && nonfinite2<false>(d2)) {
+                        d2 = 0;
+                        *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
+                    }
+                    const uint32_t w[4] = {x.w[i].x, x.w[i].y, x.w[i].z, x.w[i].w};
+                    uint32_t y[4 * OUT];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if constexpr (KIND == kKvQ8_0) {
+                            const uint32_t v = w[j] ^ 0x80808080u;
+                            y[2 * j] = h2mul(h2sub(__byte_perm(v, 0x64646464u, 0x4140), 0x64806480u), d2);
+                            y[2 * j + 1] = h2mul(h2sub(__byte_perm(v, 0x64646464u, 0x4342), 0x64806480u), d2);
+                        } else {
+                            const uint32_t a = w[j] & 0x0F0F0F0Fu, e = (w[j] >> 4) & 0x0F0F0F0Fu;
+                            y[2 * j] = h2mul(h2sub(__byte_perm(a, 0x64646464u, 0x4140), 0x64086408u), d2);
+                            y[2 * j + 1] = h2mul(h2sub(__byte_perm(a, 0x64646464u, 0x4342), 0x64086408u), d2);
+                            y[8 + 2 * j] = h2mul(h2sub(__byte_perm(e, 0x64646464u, 0x4140), 0x64086408u), d2);
+                            y[8 + 2 * j + 1] = h2mul(h2sub(__byte_perm(e, 0x64646464u, 0x4342), 0x64086408u), d2);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < OUT; ++j) {
+                        const int oc = ch * OUT + j;
+                        *reinterpret_cast<uint4 *>(dst + (oc >> 3) * (S::keys * 128) + r * 128 + (((oc & 7) ^ (r & 7)) << 4)) =
+                            make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                    }
+                }
+                announce(b);
+                ++nb;
+            };
+            while (p.b < bt.batch && p.unit0 < hi) {
+                const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                ++unit;
+                Codes ck, cv;
+                share_rows(rows_of(u, u.t0), seq);
+                fetch(ck, seq, 0);
+                for (int t = u.t0; t < u.t1; ++t, ++seq) {
+                    const bool more = t + 1 < u.t1;
+                    const int64_t row = more ? rows_of(u, t + 1) : -2;
+                    fetch(cv, seq, 1);
+                    widen(ck, false);
+                    if (more) {
+                        share_rows(row, seq + 1);
+                        fetch(ck, seq + 1, 0);
+                    }
+                    widen(cv, t * S::keys + S::keys > u.free_end);
+                }
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
+            }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 12 && lane == 0) {
+        if (warp == 12 && elect_one()) {
             // ================= products ================================================================
             constexpr uint32_t fmt = BF ? 1 : 0;
             constexpr uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
             constexpr uint32_t id_qk = idesc0 | (uint32_t(S::keys / 8) << 17);
             constexpr uint32_t id_pv = idesc0 | (1u << 16) | (uint32_t(D / 8) << 17);  // V: its columns are contiguous
-            uint32_t nb = 0, nq[2] = {0, 0}, np[2] = {0, 0};
+            uint32_t nb = 0, nq[2] = {0, 0}, np[2][2] = {};  // buffers, units, tiles by turn
+            const uint32_t q0 = smem_desc_lo(smem_u32(sq), 16), k0 = smem_desc_lo(smem_u32(sbuf), 16),
+                           v0 = smem_desc_lo(smem_u32(sbuf), S::keys * 128);
             auto qk = [&](int w, int x, uint32_t b) {
-                const uint32_t a = smem_u32(sq) + w * 128 * 128, k = smem_u32(sbuf) + b * S::buf;
+                const uint32_t a = q0 + ((w * 128 * 128) >> 4), k = k0 + b * (S::buf >> 4);
 #pragma unroll
                 for (int i = 0; i < D / 16; ++i)
-                    mma_ss(tmem + x * S::s_cols, smem_desc(a + (i >> 2) * (S::rows * 128) + (i & 3) * 32, 16, 1024),
-                           smem_desc(k + (i >> 2) * (S::keys * 128) + (i & 3) * 32, 16, 1024), id_qk, i > 0);
-                mma_commit(&sh.s_full[x]);
+                    mma_ss(tmem + (w * 2 + x) * S::s_cols, smem_desc(a + (((i >> 2) * (S::rows * 128) + (i & 3) * 32) >> 4)),
+                           smem_desc(k + (((i >> 2) * (S::keys * 128) + (i & 3) * 32) >> 4)), id_qk, i > 0);
+                mma_commit(&sh.s_full[w][x]);
             };
             auto pv = [&](int w, int x, uint32_t b, bool acc) {
-                const uint32_t v = smem_u32(sbuf) + b * S::buf;
+                const uint32_t v = v0 + b * (S::buf >> 4);
 #pragma unroll
                 for (int i = 0; i < S::keys / 16; ++i)
-                    mma_ts(tmem + S::o_col + (S::nq == 2 ? w * S::o_cols : 0), tmem + x * S::s_cols + i * 8,
-                           smem_desc(v + i * 2048, S::keys * 128, 1024), id_pv, acc || i > 0);
-                mma_commit(&sh.pv_done[w]);
+                    mma_ts(tmem + S::o_col + w * S::o_cols, tmem + (w * 2 + x) * S::s_cols + i * 8,
+                           smem_desc(v + ((i * 2048) >> 4)), id_pv, acc || i > 0);
+                mma_commit(&sh.pv_done[w][x]);
             };
             auto wait_full = [&](uint32_t n) {
                 tile_wait(&sh, &sh.full[n % S::nbuf], (n / S::nbuf) & 1, limit_ns);
@@ -576,33 +601,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                 for (int w = 0; w < S::nq; ++w)
                     if (w < active) tile_wait(&sh, &sh.q_full[w], nq[w]++ & 1, limit_ns);
-                wait_full(nb);
+                // One tile ahead of the softmax: S of tile i + 1 goes to the other turn's columns, whose P was read
+                // by the products of tile i - 1, which were issued before.
+                for (int i = -1; i < tiles; ++i) {
+                    if (i + 1 < tiles) {
+                        const uint32_t b = nb + 2 * (i + 1);
+                        wait_full(b);
 #pragma unroll
-                for (int w = 0; w < S::nq; ++w)
-                    if (w < active) qk(w, w, nb % S::nbuf);
-                mma_commit(&sh.empty[nb % S::nbuf]);
-                for (int i = 0; i < tiles; ++i) {
-                    const uint32_t bv = nb + 2 * i + 1, bk = bv + 1;
-                    const bool more = i + 1 < tiles;
-                    if (S::nq == 1 && more) {  // the next scores go to the other turn's columns
-                        wait_full(bk);
-                        qk(0, (i + 1) & 1, bk % S::nbuf);
-                        mma_commit(&sh.empty[bk % S::nbuf]);
+                        for (int w = 0; w < S::nq; ++w)
+                            if (w < active) qk(w, (i + 1) & 1, b % S::nbuf);
+                        mma_commit(&sh.empty[b % S::nbuf]);
                     }
+                    if (i < 0) continue;
+                    const uint32_t b = nb + 2 * i + 1;
+                    wait_full(b);
 #pragma unroll
-                    for (int w = 0; w < S::nq; ++w) {
-                        if (w >= active) continue;
-                        if (w == 0) wait_full(bv);
-                        tile_wait(&sh, &sh.p_full[w], np[w]++ & 1, limit_ns);
-                        fence_after();
-                        pv(w, S::nq == 2 ? w : i & 1, bv % S::nbuf, i > 0);
-                        if (S::nq == 2 && more) {
-                            if (w == 0) wait_full(bk);
-                            qk(w, w, bk % S::nbuf);
+                    for (int w = 0; w < S::nq; ++w)
+                        if (w < active) {
+                            if (i & 1) tile_wait(&sh, &sh.p_full[w][1], np[w][1]++ & 1, limit_ns);
+                            else tile_wait(&sh, &sh.p_full[w][0], np[w][0]++ & 1, limit_ns);
+                            fence_after();
+                            pv(w, i & 1, b % S::nbuf, i > 0);
                         }
-                    }
-                    mma_commit(&sh.empty[bv % S::nbuf]);
-                    if (S::nq == 2 && more) mma_commit(&sh.empty[bk % S::nbuf]);
+                    mma_commit(&sh.empty[b % S::nbuf]);
                 }
                 nb += 2 * tiles;
                 attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
@@ -637,7 +658,7 @@ template <int KIND> static int tile_dim(int D, const KvCacheView &c, const KvBat
                     : launch_tile<KIND, 256>(c, bt, io, ctas, join, s);
 }
 
-AttnTiles attn_tile_tiles(int D) { return D == 256 ? AttnTiles{128, 64, 1} : AttnTiles{256, 128, 1}; }
+AttnTiles attn_tile_tiles(int D) { return D == 256 ? AttnTiles{128, 64, 1} : AttnTiles{256, 64, 1}; }
 
 int attn_tile_launch(int kind, int D, const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas, bool join,
                      cudaStream_t s) {
