@@ -10,13 +10,15 @@
 // the last ones are done, and the softmax never waits for a product that waits for it.  (Tiles of 128
 // keys fill tensor memory with one turn, P over S: the chain softmax, P V, Q K^T, softmax then left
 // both sides idle half of the time: 2.68 against FILLCHUNK ms for 2048 rows over 30049 keys.)
-// Warp roles: warps 0-3 and 4-7 are the softmax of the two row tiles; warps 8-11 bring keys and values through
-// the page table into a ring of buffers in the 128-byte swizzled layout, widening quantised codes
-// to fp16 on the way; warp 12 issues every product.  All hand-over is by mbarriers; each wait is
-// bounded and a failure makes the later ones return at once.
+// Warp roles: warps 0-3 and 4-7 are the softmax of the two row tiles; warps 8-14 bring keys and values
+// through the page table into rings of buffers in the 128-byte swizzled layout, widening quantised
+// codes to fp16 on the way; warp 15 issues every product.  All hand-over is by mbarriers; each wait is bounded and
+// a failure makes the later ones return at once.
 //
 // The running maximum is only raised when it grew by more than 2^8 (weights may then reach 2^8, which
 // fp16 and fp32 hold without loss), so that O is rescaled a few times a row instead of at every tile.
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "anvil.h"
@@ -25,7 +27,8 @@
 
 namespace anvil {
 
-constexpr int kTileThreads = 512;
+constexpr int kTileThreads = 512;   // 128 registers a thread at launch, divided anew by warp group below
+constexpr int kTileLoaders = 224;   // threads of the seven loading warps
 constexpr int kTileCost = 8;        // beginning and ending a unit, in key tiles
 constexpr float kTileSlack = 8.0f;  // log2 of how far weights may exceed 1
 
@@ -36,8 +39,8 @@ template <int KIND, int D> struct TileShape {
     static constexpr int blocks = D / 64;               // 64-value column blocks of an operand
     static constexpr int q_bytes = rows * D * 2;
     static constexpr int buf = keys * D * 2;            // one buffer: keys or values of a tile
-    static constexpr int nbuf = D == 256 ? 4 : 8;
-    static constexpr int smem = 1024 + q_bytes + nbuf * buf;
+    static constexpr int nbuf = D == 256 ? 2 : 4;       // buffers of keys, and of values
+    static constexpr int smem = 1024 + q_bytes + 2 * nbuf * buf;
     static constexpr bool bf16 = KIND == kKvBF16;
     static constexpr bool quant = KIND == kKvQ8_0 || KIND == kKvQ4_0;
     // tensor memory columns: two turns of S for each row tile, then O
@@ -106,12 +109,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
 
 struct TileShared {
     AttnScratch sc;
-    uint64_t full[8], empty[8], q_full[2], s_full[2][2], p_full[2][2], pv_done[2][2], drain;  // [row tile][turn]
+    uint64_t full[2][4], empty[2][4], q_full[2],  // [keys, values][buffer]
+         s_full[2][2], p_full[2][2], pv_done[2][2], drain;  // [row tile][turn]
     uint32_t tmem;
     int failed;             // a wait gave up: later ones do not wait
     int dirty[8];           // [unit % 8] = unit where non-finite values were taken out of its value tiles
     uint32_t bad[8][2];     // [tile % 8]: keys without a page
-    int64_t row[2][64];    // loader: cache rows of a key tile, by parity
 };
 
 // Bounded by the wall clock, which is only looked at after some hundred polls: reading it takes longer
@@ -131,7 +134,20 @@ __device__ __forceinline__ void tile_wait(TileShared *sh, uint64_t *bar, uint32_
         }
     }
 }
-__device__ __forceinline__ void loader_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// Whether a phase is over, without the wait that try_wait may take.
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+// A box of 64 columns from (x, y) of a tensor of 16-bit rows into the 128-byte swizzled layout.
+__device__ __forceinline__ void tma_box(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                     smem_u32(dst)),
+                 "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+                 : "memory");
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // A unit's share of this CTA: key tiles [t0, t1) and the limits of its masks.
@@ -154,7 +170,8 @@ template <int KIND, int D> struct TileUnit {
 
 template <int KIND, int D>
 __global__ void __launch_bounds__(kTileThreads, 1)
-    attn_tile_kernel(KvCacheView c, KvBatchView bt, AttnIO io, uint64_t limit_ns) {
+    attn_tile_kernel(KvCacheView c, KvBatchView bt, AttnIO io, const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v, int box, uint64_t limit_ns) {
     using S = TileShape<KIND, D>;
     constexpr bool BF = S::bf16;
     extern __shared__ uint8_t dyn[];
@@ -172,10 +189,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     AttnPos p = sh.sc.pos;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::nbuf; ++i) {
-            mbar_init(&sh.full[i], 4);
-            mbar_init(&sh.empty[i], 1);
-        }
+        for (int i = 0; i < S::nbuf; ++i)
+            for (int kv = 0; kv < 2; ++kv) {
+                mbar_init(&sh.full[kv][i], kTileLoaders / 32);
+                mbar_init(&sh.empty[kv][i], 1);
+            }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.q_full[i], 4);
             for (int x = 0; x < 2; ++x) {
@@ -189,7 +207,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         sh.failed = 0;
         for (int i = 0; i < 8; ++i) sh.dirty[i] = 0;
     }
-    if (warp == 12) {
+    if (warp == 15) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         fence_before();
@@ -198,9 +216,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&sh.tmem);
 
+    // Registers by warp group: 2 x 160 + 2 x 96 = 4 x 128, what the CTA was launched with.
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if (warp < 8) {
         // ================= softmax: thread = row of tile w ==========================================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
         const int w = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         // Tiles so far on each turn.  S, P and P V of a tile use its turn's barriers: a side may be a whole tile
@@ -385,93 +405,135 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 seq += u.t1 - u.t0;
                 attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
             }
-    } else if (warp < 12) {
-        // ================= loader: 128 threads, keys then values of each tile ========================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    } else if (warp < 15) {
+        // ================= loaders: keys and values of a tile together ===============================
+        constexpr int LT = kTileLoaders;
         const int tid = threadIdx.x - 256;
-        uint32_t nb = 0;        // buffers filled
-        int unit = 0, seq = 0;
-        auto announce = [&](int b) {
+        int unit = 0, seq = 0;  // units and tiles begun
+        auto announce = [&](int kv, int b) {
             fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.full[b]);
+            if (lane == 0) mbar_arrive(&sh.full[kv][b]);
         };
-        // cache rows of key tile t, key by key, for everyone; rows of the keys behind the last: -2
-        auto rows_of = [&](const TileUnit<KIND, D> &u, int t) -> int64_t {
-            const int key = t * S::keys + tid;
-            return tid < S::keys && key < u.key_end ? kv_lookup(bt, c, p.b, key, p.head) : -2;
+        // Page of a key (0 behind the last one), looked up a tile ahead of its use; and the key's cache row, -1 where
+        // there is no page and -2 behind the last key.
+        auto page_of = [&](const TileUnit<KIND, D> &u, int key) {
+            return key < u.key_end ? __ldg(bt.table + p.b * bt.table_stride + (key >> c.page_shift)) : 0;
         };
-        auto share_rows = [&](int64_t row, int at) {
-            const uint32_t bad = __ballot_sync(0xffffffffu, row == -1);
-            if (tid < S::keys) {
-                sh.row[at & 1][tid] = row;
-                if (lane == 0) {
-                    sh.bad[at & 7][tid >> 5] = bad;
-                    if (bad) flag_bad_page();
-                }
+        auto row_of = [&](const TileUnit<KIND, D> &u, int key, int page) -> int64_t {
+            return key < u.key_end
+                       ? kv_row(page, c.num_pages, p.head, c.kv_heads, key & ((1 << c.page_shift) - 1), c.page_shift)
+                       : -2;
+        };
+        // keys of the tile without a page, for the softmax (each of the first two warps knows 32 of them)
+        auto share_bad = [&](bool none) {
+            const uint32_t bad = __ballot_sync(0xffffffffu, none);
+            if (tid < S::keys && lane == 0) {
+                sh.bad[seq & 7][tid >> 5] = bad;
+                if (bad) flag_bad_page();
             }
-            loader_sync();
+        };
+        // place of 16-byte chunk oc of key r in a buffer
+        auto place = [&](int kv, int b, int r, int oc) {
+            return sbuf + (kv * S::nbuf + b) * S::buf + (oc >> 3) * (S::keys * 128) + r * 128 + (((oc & 7) ^ (r & 7)) << 4);
         };
         if constexpr (!S::quant) {
-            // 16-bit rows go straight to their places; up to `depth` buffers' copies are in flight, announced in order
-            constexpr int CH = D / 8, depth = S::nbuf / 2;
+            // 16-bit rows go straight to their places.  A tile that every row sees whole, in pages of 8 keys and more,
+            // is copied by TMA, a box of up to 64 keys of one page and 64 columns at a time; others by cp.async, whose
+            // tiles are announced when the next one's copies are on their way.
+            constexpr int CH = D / 8, ALL = 2 * S::keys * CH, depth = S::nbuf > 2 ? 2 : 1;
+            const int boxes = box ? S::keys / box : 0;  // of a tile's keys; box 0: no TMA
             int pending = 0;
-            auto settle = [&](int left) {  // all copies are done: announce all but the newest `left`
-                for (; pending > left; --pending) announce((nb - pending) % S::nbuf);
+            auto settle = [&](int left) {  // announces all but the newest `left` tiles, whose copies are done
+                for (; pending > left; --pending) {
+                    const int b = (seq - pending) % S::nbuf;
+                    announce(0, b);
+                    if (lane == 0) mbar_arrive(&sh.full[1][b]);
+                }
             };
             while (p.b < bt.batch && p.unit0 < hi) {
                 const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
                 ++unit;
-                int64_t row = rows_of(u, u.t0);
-                for (int t = u.t0; t < u.t1; ++t, ++seq) {
-                    share_rows(row, seq);
-                    if (t + 1 < u.t1) row = rows_of(u, t + 1);
-                    const bool check = t * S::keys + S::keys > u.free_end;
-                    for (int kv = 0; kv < 2; ++kv) {
-                        const int b = nb % S::nbuf;
-                        if (nb >= S::nbuf) {
-                            const uint32_t parity = (nb / S::nbuf - 1) & 1;
-                            // (a product may wait for a pending buffer before it frees this one)
-                            if (pending && !__all_sync(0xffffffffu, mbar_try_wait(&sh.empty[b], parity))) {
-                                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                                settle(0);
-                            }
-                            tile_wait(&sh, &sh.empty[b], parity, limit_ns);
+                // lane i: the page of box i
+                int page = lane < boxes ? page_of(u, u.t0 * S::keys + lane * box) : 0;
+                for (int t = u.t0; t < u.t1; ++t) {
+                    const bool check = (t + 1) * S::keys > u.free_end;
+                    const int64_t row = lane < boxes ? row_of(u, t * S::keys + lane * box, page) : 0;
+                    const bool fast = boxes && !check && !__any_sync(0xffffffffu, row < 0);
+                    if (lane < boxes && t + 1 < u.t1) page = page_of(u, (t + 1) * S::keys + lane * box);
+                    const int b = seq % S::nbuf;
+                    const uint32_t parity = (seq / S::nbuf - 1) & 1;
+                    // (a product may wait for a pending tile before it frees this one's buffers)
+                    if (pending && (fast || !__all_sync(0xffffffffu, seq < S::nbuf || mbar_test(&sh.empty[1][b], parity)))) {
+                        asm volatile("cp.async.wait_group 0;" ::: "memory");
+                        settle(0);
+                    }
+                    if (seq >= S::nbuf) {
+                        tile_wait(&sh, &sh.empty[0][b], parity, limit_ns);
+                        tile_wait(&sh, &sh.empty[1][b], parity, limit_ns);
+                        __syncwarp();
+                    }
+                    if (fast) {
+                        share_bad(false);
+                        if (warp == 8) {
                             __syncwarp();
-                        }
-                        uint8_t *dst = sbuf + b * S::buf;
-                        const uint8_t *src = kv ? c.v : c.k;
+                            for (int i = 0; i < boxes; ++i) {
+                                const int y = int(__shfl_sync(0xffffffffu, row, i));
+                                if (elect_one()) {
+                                    if (i == 0) {
+                                        mbar_arrive_expect_tx(&sh.full[0][b], S::buf);
+                                        mbar_arrive_expect_tx(&sh.full[1][b], S::buf);
+                                    }
 #pragma unroll
-                        for (int i = 0; i < S::keys * CH / 128; ++i) {
-                            const int r = tid / CH + i * (128 / CH), ch = tid % CH;
-                            const int64_t rw = sh.row[seq & 1][r];
-                            const uint32_t to = smem_u32(dst + (ch >> 3) * (S::keys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to),
-                                         "l"(src + max(rw, int64_t(0)) * (2 * D) + ch * 16), "r"(rw < 0 ? 0 : 16)
-                                         : "memory");
-                        }
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        ++nb;
-                        ++pending;
-                        if (kv && check) {
-                            // a masked tile's values: what is not finite leaves the product (see the outputs)
-                            asm volatile("cp.async.wait_group 0;" ::: "memory");
-                            for (int i = 0; i < S::keys * CH / 128; ++i) {
-                                const int r = tid / CH + i * (128 / CH), ch = tid % CH;
-                                uint4 *w4 = reinterpret_cast<uint4 *>(dst + (ch >> 3) * (S::keys * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
-                                uint4 x = *w4;
-                                const uint32_t n[4] = {nonfinite2<BF>(x.x), nonfinite2<BF>(x.y), nonfinite2<BF>(x.z), nonfinite2<BF>(x.w)};
-                                if (n[0] | n[1] | n[2] | n[3]) {
-                                    *w4 = make_uint4(x.x & ~n[0], x.y & ~n[1], x.z & ~n[2], x.w & ~n[3]);
-                                    *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
+                                    for (int j = 0; j < S::blocks; ++j) {
+                                        tma_box(place(0, b, i * box, 8 * j), &map_k, 64 * j, y, &sh.full[0][b]);
+                                        tma_box(place(1, b, i * box, 8 * j), &map_v, 64 * j, y, &sh.full[1][b]);
+                                    }
                                 }
+                                __syncwarp();
                             }
-                            __syncwarp();
-                            settle(0);
-                        } else if (pending == depth) {
-                            asm volatile("cp.async.wait_group %0;" ::"n"(depth - 1) : "memory");
-                            settle(depth - 1);
+                        } else if (lane == 0) {
+                            mbar_arrive(&sh.full[0][b]);
+                            mbar_arrive(&sh.full[1][b]);
                         }
+                        ++seq;
+                        continue;
+                    }
+                    {
+                        const int key = t * S::keys + tid;
+                        share_bad(tid < S::keys && row_of(u, key, page_of(u, key)) == -1);
+                    }
+#pragma unroll
+                    for (int i = 0; i < (ALL + LT - 1) / LT; ++i) {
+                        const int at = tid + i * LT, kv = at / (ALL / 2), r = at / CH % S::keys, ch = at % CH;
+                        if (at >= ALL) break;
+                        const int64_t rw = row_of(u, t * S::keys + r, page_of(u, t * S::keys + r));
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(place(kv, b, r, ch))),
+                                     "l"((kv ? c.v : c.k) + max(rw, int64_t(0)) * (2 * D) + ch * 16), "r"(rw < 0 ? 0 : 16)
+                                     : "memory");
+                    }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    ++seq;
+                    ++pending;
+                    if (check) {
+                        // a masked tile's values: what is not finite leaves the product (see the outputs)
+                        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll 1
+                        for (int at = tid; at < ALL; at += LT) {
+                            if (at < ALL / 2) continue;
+                            uint4 *w4 = reinterpret_cast<uint4 *>(place(1, b, at / CH % S::keys, at % CH));
+                            const uint4 x = *w4;
+                            const uint32_t n[4] = {nonfinite2<BF>(x.x), nonfinite2<BF>(x.y), nonfinite2<BF>(x.z), nonfinite2<BF>(x.w)};
+                            if (n[0] | n[1] | n[2] | n[3]) {
+                                *w4 = make_uint4(x.x & ~n[0], x.y & ~n[1], x.z & ~n[2], x.w & ~n[3]);
+                                *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
+                            }
+                        }
+                        __syncwarp();
+                        settle(0);
+                    } else if (pending == depth) {
+                        asm volatile("cp.async.wait_group %0;" ::"n"(depth - 1) : "memory");
+                        settle(depth - 1);
                     }
                 }
                 attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
@@ -479,55 +541,82 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             settle(0);
         } else {
-            // 16 bytes of codes a turn: 16 (Q8_0) or 32 (Q4_0) values, two or four chunks of 16 bytes.  The next
-            // buffer's codes are in flight while this one's are widened.
-            constexpr int RB = KvRow<KIND, D>::bytes, CH = RB / 16, N = S::keys * CH / 128;
+            // 16 bytes of codes a turn: 16 (Q8_0) or 32 (Q4_0) values, two or four chunks.  A job, the keys and values
+            // of a tile (of D = 256, Q8_0: either), is fetched while the job before is widened, and only after
+            // that one's codes have arrived.
+            constexpr int RB = KvRow<KIND, D>::bytes, CH = RB / 16, HALF = S::keys * CH;
+            constexpr int jobs = CH > 8 ? 2 : 1, ALL = 2 * HALF / jobs, N = (ALL + LT - 1) / LT;
             constexpr int OUT = KIND == kKvQ8_0 ? 2 : 4, VALS = 8 * OUT;
-            // eight lanes store two rows of four chunks where rows have them: distinct banks
-            const int in = tid % (2 * CH);
-            const int ch = CH >= 8 ? (in & 3) | ((in >> 3) << 2) : tid % CH;
-            const int r0 = CH >= 8 ? tid / (2 * CH) * 2 + ((in >> 2) & 1) : tid / CH;
-            struct Codes {
-                uint4 w[N];
-                uint32_t d[N];
+            uint4 w[N], wn[N];
+            uint32_t d[N], dn[N], gone = 0;  // gone: bits of the fetched chunks whose key is not there
+            int pages[N], own = 0;           // pages of the next fetch's keys, and of key `tid`
+            // the i-th chunk of this thread: (keys or values, key, chunk); eight lanes store two rows of four
+            // chunks where rows have them: distinct banks
+            auto item = [&](int i, int job, int &kv, int &r, int &ch) {
+                const int at = min(tid + i * LT, ALL - 1) + job * ALL, j = at % HALF, in = j % (2 * CH);
+                kv = at / HALF;
+                ch = CH >= 8 ? (in & 3) | ((in >> 3) << 2) : j % CH;
+                r = CH >= 8 ? j / (2 * CH) * 2 + ((in >> 2) & 1) : j / CH;
+                return tid + i * LT < ALL;
             };
-            auto fetch = [&](Codes &x, int at, int kv) {
-                const uint8_t *src = kv ? c.v : c.k;
-                const unsigned short *scales = reinterpret_cast<const unsigned short *>(kv ? c.vs : c.ks);
+            // Loads without a condition (of the pool's first row where there is none): loads in branches would be
+            // waited for one after the other.
+            auto look = [&](const TileUnit<KIND, D> &u, int t, int job) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int64_t rw = sh.row[at & 1][r0 + i * (128 / CH)];
-                    x.w[i] = make_uint4(0, 0, 0, 0);
-                    x.d[i] = 0;
-                    if (rw >= 0) {
-                        x.w[i] = __ldg(reinterpret_cast<const uint4 *>(src + rw * RB + ch * 16));
-                        x.d[i] = __ldg(scales + rw * (D / 32) + ch * VALS / 32);
-                    }
+                    int kv, r, ch;
+                    item(i, job, kv, r, ch);
+                    pages[i] = page_of(u, t * S::keys + r);
+                }
+                if (job == 0) own = page_of(u, t * S::keys + tid);
+            };
+            auto fetch = [&](const TileUnit<KIND, D> &u, int t, int job) {
+                gone = 0;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    int kv, r, ch;
+                    item(i, job, kv, r, ch);
+                    const int64_t rw = row_of(u, t * S::keys + r, pages[i]);
+                    gone |= rw < 0 ? 1u << i : 0;
+                    const int64_t row = max(rw, int64_t(0));
+                    wn[i] = __ldg(reinterpret_cast<const uint4 *>((kv ? c.v : c.k) + row * RB + ch * 16));
+                    dn[i] = __ldg(reinterpret_cast<const unsigned short *>(kv ? c.vs : c.ks) + row * (D / 32) + ch * VALS / 32);
                 }
             };
-            auto widen = [&](const Codes &x, bool check) {
-                const int b = nb % S::nbuf;
-                if (nb >= S::nbuf) tile_wait(&sh, &sh.empty[b], (nb / S::nbuf - 1) & 1, limit_ns);
-                __syncwarp();
-                uint8_t *dst = sbuf + b * S::buf;
+            auto take = [&]() {  // the fetched codes, that is, waits for them
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int r = r0 + i * (128 / CH);
-                    uint32_t d2 = dup16(x.d[i]);
-                    if (check && nonfinite2<false>(d2)) {
+                    constexpr uint32_t flip = KIND == kKvQ8_0 ? 0x80808080u : 0;
+                    w[i] = make_uint4(wn[i].x ^ flip, wn[i].y ^ flip, wn[i].z ^ flip, wn[i].w ^ flip);
+                    d[i] = (gone >> i) & 1 ? 0 : dup16(dn[i]);
+                }
+            };
+            auto widen = [&](int job, bool check) {
+                const int b = seq % S::nbuf;
+                if (seq >= S::nbuf) {
+                    const uint32_t parity = (seq / S::nbuf - 1) & 1;
+                    if (jobs == 1 || job == 0) tile_wait(&sh, &sh.empty[0][b], parity, limit_ns);
+                    if (jobs == 1 || job == 1) tile_wait(&sh, &sh.empty[1][b], parity, limit_ns);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    int kv, r, ch;
+                    if (!item(i, job, kv, r, ch)) break;
+                    uint32_t d2 = d[i];
+                    if (check && kv && nonfinite2<false>(d2)) {
                         d2 = 0;
                         *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
                     }
-                    const uint32_t w[4] = {x.w[i].x, x.w[i].y, x.w[i].z, x.w[i].w};
+                    const uint32_t x[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
                     uint32_t y[4 * OUT];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        if constexpr (KIND == kKvQ8_0) {
-                            const uint32_t v = w[j] ^ 0x80808080u;
-                            y[2 * j] = h2mul(h2sub(__byte_perm(v, 0x64646464u, 0x4140), 0x64806480u), d2);
-                            y[2 * j + 1] = h2mul(h2sub(__byte_perm(v, 0x64646464u, 0x4342), 0x64806480u), d2);
+                        if constexpr (KIND == kKvQ8_0) {  // x: codes + 128
+                            y[2 * j] = h2mul(h2sub(__byte_perm(x[j], 0x64646464u, 0x4140), 0x64806480u), d2);
+                            y[2 * j + 1] = h2mul(h2sub(__byte_perm(x[j], 0x64646464u, 0x4342), 0x64806480u), d2);
                         } else {
-                            const uint32_t a = w[j] & 0x0F0F0F0Fu, e = (w[j] >> 4) & 0x0F0F0F0Fu;
+                            const uint32_t a = x[j] & 0x0F0F0F0Fu, e = (x[j] >> 4) & 0x0F0F0F0Fu;
                             y[2 * j] = h2mul(h2sub(__byte_perm(a, 0x64646464u, 0x4140), 0x64086408u), d2);
                             y[2 * j + 1] = h2mul(h2sub(__byte_perm(a, 0x64646464u, 0x4342), 0x64086408u), d2);
                             y[8 + 2 * j] = h2mul(h2sub(__byte_perm(e, 0x64646464u, 0x4140), 0x64086408u), d2);
@@ -535,46 +624,51 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < OUT; ++j) {
-                        const int oc = ch * OUT + j;
-                        *reinterpret_cast<uint4 *>(dst + (oc >> 3) * (S::keys * 128) + r * 128 + (((oc & 7) ^ (r & 7)) << 4)) =
+                    for (int j = 0; j < OUT; ++j)
+                        *reinterpret_cast<uint4 *>(place(kv, b, r, ch * OUT + j)) =
                             make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
-                    }
                 }
-                announce(b);
-                ++nb;
+                announce(jobs == 1 ? 0 : job, b);
+                if (jobs == 1 && lane == 0) mbar_arrive(&sh.full[1][b]);
             };
             while (p.b < bt.batch && p.unit0 < hi) {
                 const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
                 ++unit;
-                Codes ck, cv;
-                share_rows(rows_of(u, u.t0), seq);
-                fetch(ck, seq, 0);
-                for (int t = u.t0; t < u.t1; ++t, ++seq) {
-                    const bool more = t + 1 < u.t1;
-                    const int64_t row = more ? rows_of(u, t + 1) : -2;
-                    fetch(cv, seq, 1);
-                    widen(ck, false);
-                    if (more) {
-                        share_rows(row, seq + 1);
-                        fetch(ck, seq + 1, 0);
+                look(u, u.t0, 0);
+                fetch(u, u.t0, 0);
+                int mine = own;  // page of key `tid` of tile t
+                look(u, jobs == 2 ? u.t0 : u.t0 + 1, jobs - 1);
+                for (int t = u.t0; t < u.t1; ++t) {
+                    const bool check = (t + 1) * S::keys > u.free_end, more = t + 1 < u.t1;
+                    share_bad(tid < S::keys && row_of(u, t * S::keys + tid, mine) == -1);
+                    take();
+                    if (jobs == 2) {
+                        fetch(u, t, 1);
+                        look(u, t + 1, 0);
+                        widen(0, false);
+                        take();
                     }
-                    widen(cv, t * S::keys + S::keys > u.free_end);
+                    mine = own;
+                    if (more) {
+                        fetch(u, t + 1, 0);
+                        look(u, jobs == 2 ? t + 1 : t + 2, jobs - 1);
+                    }
+                    widen(jobs - 1, check);
+                    ++seq;
                 }
                 attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
             }
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 12 && elect_one()) {
+        if (elect_one()) {
             // ================= products ================================================================
             constexpr uint32_t fmt = BF ? 1 : 0;
             constexpr uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
             constexpr uint32_t id_qk = idesc0 | (uint32_t(S::keys / 8) << 17);
             constexpr uint32_t id_pv = idesc0 | (1u << 16) | (uint32_t(D / 8) << 17);  // V: its columns are contiguous
-            uint32_t nb = 0, nq[2] = {0, 0}, np[2][2] = {};  // buffers, units, tiles by turn
+            uint32_t nb = 0, nq[2] = {0, 0}, np[2][2] = {};  // tiles, units, tiles by turn
             const uint32_t q0 = smem_desc_lo(smem_u32(sq), 16), k0 = smem_desc_lo(smem_u32(sbuf), 16),
-                           v0 = smem_desc_lo(smem_u32(sbuf), S::keys * 128);
+                           v0 = smem_desc_lo(smem_u32(sbuf + S::nbuf * S::buf), S::keys * 128);
             auto qk = [&](int w, int x, uint32_t b) {
                 const uint32_t a = q0 + ((w * 128 * 128) >> 4), k = k0 + b * (S::buf >> 4);
 #pragma unroll
@@ -591,8 +685,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                            smem_desc(v + ((i * 2048) >> 4)), id_pv, acc || i > 0);
                 mma_commit(&sh.pv_done[w][x]);
             };
-            auto wait_full = [&](uint32_t n) {
-                tile_wait(&sh, &sh.full[n % S::nbuf], (n / S::nbuf) & 1, limit_ns);
+            auto wait_full = [&](int kv, uint32_t n) {
+                tile_wait(&sh, &sh.full[kv][n % S::nbuf], (n / S::nbuf) & 1, limit_ns);
                 fence_after();
             };
             while (p.b < bt.batch && p.unit0 < hi) {
@@ -605,16 +699,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 // by the products of tile i - 1, which were issued before.
                 for (int i = -1; i < tiles; ++i) {
                     if (i + 1 < tiles) {
-                        const uint32_t b = nb + 2 * (i + 1);
-                        wait_full(b);
+                        const uint32_t b = nb + i + 1;
+                        wait_full(0, b);
 #pragma unroll
                         for (int w = 0; w < S::nq; ++w)
                             if (w < active) qk(w, (i + 1) & 1, b % S::nbuf);
-                        mma_commit(&sh.empty[b % S::nbuf]);
+                        mma_commit(&sh.empty[0][b % S::nbuf]);
                     }
                     if (i < 0) continue;
-                    const uint32_t b = nb + 2 * i + 1;
-                    wait_full(b);
+                    const uint32_t b = nb + i;
+                    wait_full(1, b);
 #pragma unroll
                     for (int w = 0; w < S::nq; ++w)
                         if (w < active) {
@@ -623,9 +717,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             fence_after();
                             pv(w, i & 1, b % S::nbuf, i > 0);
                         }
-                    mma_commit(&sh.empty[b % S::nbuf]);
+                    mma_commit(&sh.empty[1][b % S::nbuf]);
                 }
-                nb += 2 * tiles;
+                nb += tiles;
                 attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
             }
             mma_commit(&sh.drain);
@@ -635,10 +729,32 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 15) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
+}
+
+// Tensor map of a 16-bit cache tensor as rows of D values, read in boxes of `box` rows and 64 columns.
+static int tile_map(CUtensorMap *map, void *data, int D, int64_t rows, int box) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        return cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found) == cudaSuccess &&
+                       found == cudaDriverEntryPointSuccess
+                   ? reinterpret_cast<Encode>(f)
+                   : nullptr;
+    }();
+    if (!encode) return fail(ANVIL_ERR_CUDA, "cuTensorMapEncodeTiled not found");
+    const cuuint64_t dims[2] = {cuuint64_t(D), cuuint64_t(rows)}, strides[1] = {cuuint64_t(2 * D)};
+    const cuuint32_t boxes[2] = {64, cuuint32_t(box)}, steps[2] = {1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, data, dims, strides, boxes, steps,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? ANVIL_OK : fail(ANVIL_ERR_CUDA, "cuTensorMapEncodeTiled: error %d", int(r));
 }
 
 template <int KIND, int D> static int launch_tile(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
@@ -646,7 +762,22 @@ template <int KIND, int D> static int launch_tile(const KvCacheView &c, const Kv
     using S = TileShape<KIND, D>;
     cudaError_t e = cudaFuncSetAttribute(attn_tile_kernel<KIND, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
-    attn_tile_kernel<KIND, D><<<ctas, kTileThreads, S::smem, stream>>>(c, bt, io, wait_limit_ns());
+    // The warp groups' shares of the registers add up to 128 a thread: a build with fewer must not be launched
+    // (the group that asks for more would wait for ever).
+    static const int regs = [] {
+        cudaFuncAttributes a;
+        return cudaFuncGetAttributes(&a, attn_tile_kernel<KIND, D>) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (regs <= 120) return fail(ANVIL_ERR_UNSUPPORTED, "attention tile kernel built with %d registers", regs);
+    CUtensorMap mk = {}, mv = {};
+    const int64_t rows = (int64_t(c.num_pages) * c.kv_heads) << c.page_shift;
+    int box = 0;  // TMA takes 16-bit rows, whole swizzle atoms of 8 keys, and 31-bit row numbers
+    if (!S::quant && c.page_shift >= 3 && rows <= 0x7fffffff) {
+        box = std::min(S::keys, 1 << c.page_shift);
+        if (int st = tile_map(&mk, c.k, D, rows, box)) return st;
+        if (int st = tile_map(&mv, c.v, D, rows, box)) return st;
+    }
+    attn_tile_kernel<KIND, D><<<ctas, kTileThreads, S::smem, stream>>>(c, bt, io, mk, mv, box, wait_limit_ns());
     if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "paged_attention launch");
     return join ? attn_join_launch<S::rows, S::keys, kTileCost, D>(c, bt, io, ctas, stream) : ANVIL_OK;
 }
