@@ -223,10 +223,11 @@ __device__ __forceinline__ int64_t attn_locate(const KvCacheView &c, const KvBat
     return work;
 }
 
-// The unit behind p's; b reaches bt.batch behind the last.
+// The unit behind p's; b reaches bt.batch behind the last.  (The sequence is looked up again rather than kept in
+// registers through a unit.)
 template <int ROWS, int KEYS, int COST>
-__device__ __forceinline__ void attn_next(const KvCacheView &c, const KvBatchView &bt, AttnPos &p,
-                                          const AttnSeq<ROWS, KEYS> &q) {
+__device__ __forceinline__ void attn_next(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, AttnPos &p) {
+    const AttnSeq<ROWS, KEYS> q(load_seq(bt, c, p.b), io);
     p.unit0 += q.key_tiles(p.mt) + COST;
     if (++p.mt < q.tiles) return;
     p.mt = 0;

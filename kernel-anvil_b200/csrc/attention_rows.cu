@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
             }
         }
         __syncthreads();  // before the rings are filled again
-        attn_next<ROWS, kRowsKeys, kRowsCost>(c, bt, p, q);
+        attn_next<ROWS, kRowsKeys, kRowsCost>(c, bt, io, p);
     }
 }
 

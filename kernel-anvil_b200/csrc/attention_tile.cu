@@ -10,9 +10,9 @@
 // the last ones are done, and the softmax never waits for a product that waits for it.  (Tiles of 128
 // keys fill tensor memory with one turn, P over S: the chain softmax, P V, Q K^T, softmax then left
 // both sides idle half of the time: 2.68 against FILLCHUNK ms for 2048 rows over 30049 keys.)
-// Warp roles: warps 0-3 and 4-7 are the softmax of the two row tiles; warps 8-14 bring keys and values
+// Warp roles: warps 0-3 and 4-7 are the softmax of the two row tiles; warps 8-11 bring keys and values
 // through the page table into rings of buffers in the 128-byte swizzled layout, widening quantised
-// codes to fp16 on the way; warp 15 issues every product.  All hand-over is by mbarriers; each wait is bounded and
+// codes to fp16 on the way; warp 12 issues every product.  All hand-over is by mbarriers; each wait is bounded and
 // a failure makes the later ones return at once.
 //
 // The running maximum is only raised when it grew by more than 2^8 (weights may then reach 2^8, which
@@ -28,8 +28,9 @@
 namespace anvil {
 
 constexpr int kTileThreads = 512;   // 128 registers a thread at launch, divided anew by warp group below
-constexpr int kTileLoaders = 224;   // threads of the seven loading warps
+constexpr int kTileLoaders = 128;   // threads of the four loading warps
 constexpr int kTileCost = 8;        // beginning and ending a unit, in key tiles
+constexpr int kTileBulkShift = 4;   // pages of 16 keys: their scales are whole 16-byte pieces
 constexpr float kTileSlack = 8.0f;  // log2 of how far weights may exceed 1
 
 template <int KIND, int D> struct TileShape {
@@ -39,10 +40,15 @@ template <int KIND, int D> struct TileShape {
     static constexpr int blocks = D / 64;               // 64-value column blocks of an operand
     static constexpr int q_bytes = rows * D * 2;
     static constexpr int buf = keys * D * 2;            // one buffer: keys or values of a tile
-    static constexpr int nbuf = D == 256 ? 2 : 4;       // buffers of keys, and of values
-    static constexpr int smem = 1024 + q_bytes + 2 * nbuf * buf;
     static constexpr bool bf16 = KIND == kKvBF16;
     static constexpr bool quant = KIND == kKvQ8_0 || KIND == kKvQ4_0;
+    static constexpr int nbuf = D == 256 ? 2 : D == 128 && quant ? 3 : 4;  // buffers of keys, and of values
+    // quantised: a tile's codes and scales as they are in the cache, keys and values together (D = 256: a job each)
+    static constexpr int jobs = D == 256 ? 2 : 1;
+    static constexpr int rb = KvRow<KIND, D>::bytes, sb = KvRow<KIND, D>::scales * 2;
+    static constexpr int raw = quant ? keys * (rb + sb) * 2 / jobs : 0;
+    static constexpr int nraw = D == 256 && KIND == kKvQ8_0 ? 1 : 3;
+    static constexpr int smem = 1024 + q_bytes + 2 * nbuf * buf + nraw * raw;
     // tensor memory columns: two turns of S for each row tile, then O
     static constexpr int s_cols = keys, o_col = 4 * keys, o_cols = D;
 };
@@ -109,7 +115,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
 
 struct TileShared {
     AttnScratch sc;
-    uint64_t full[2][4], empty[2][4], q_full[2],  // [keys, values][buffer]
+    uint64_t full[2][4], empty[2][4], raw_full[3], raw_empty[3], q_full[2],  // [keys, values][buffer]
          s_full[2][2], p_full[2][2], pv_done[2][2], drain;  // [row tile][turn]
     uint32_t tmem;
     int failed;             // a wait gave up: later ones do not wait
@@ -140,6 +146,17 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
     asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
                  : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
     return ok != 0;
+}
+// Loads that leave no line in L1, which is small beside this kernel's shared memory and holds what registers do not.
+__device__ __forceinline__ uint4 ld_stream(const uint8_t *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_stream16(const uint8_t *p) {
+    uint16_t v;
+    asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(v) : "l"(p));
+    return v;
 }
 // A box of 64 columns from (x, y) of a tensor of 16-bit rows into the 128-byte swizzled layout.
 __device__ __forceinline__ void tma_box(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
@@ -177,7 +194,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     extern __shared__ uint8_t dyn[];
     __shared__ TileShared sh;
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~uintptr_t(1023));
-    uint8_t *sq = base, *sbuf = base + S::q_bytes;
+    uint8_t *sq = base, *sbuf = base + S::q_bytes, *sraw = sbuf + 2 * S::nbuf * S::buf;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     const int64_t work = attn_locate<S::rows, S::keys, kTileCost>(
@@ -194,6 +211,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 mbar_init(&sh.full[kv][i], kTileLoaders / 32);
                 mbar_init(&sh.empty[kv][i], 1);
             }
+        for (int i = 0; i < S::nraw; ++i) {
+            mbar_init(&sh.raw_full[i], 1);
+            mbar_init(&sh.raw_empty[i], kTileLoaders / 32);
+        }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sh.q_full[i], 4);
             for (int x = 0; x < 2; ++x) {
@@ -207,7 +228,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         sh.failed = 0;
         for (int i = 0; i < 8; ++i) sh.dirty[i] = 0;
     }
-    if (warp == 15) {
+    if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         fence_before();
@@ -216,9 +237,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     fence_after();
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&sh.tmem);
 
-    // Registers by warp group: 2 x 160 + 2 x 96 = 4 x 128, what the CTA was launched with.
-    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    // Registers by warp group: 2 x 152 + 136 + 72 = 4 x 128, what the CTA was launched with.
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    else if (warp < 12) asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp < 8) {
         // ================= softmax: thread = row of tile w ==========================================
         const int w = warp >> 2, r = threadIdx.x & 127;
@@ -403,9 +425,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     fence_before();
                 }
                 seq += u.t1 - u.t0;
-                attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
             }
-    } else if (warp < 15) {
+    } else if (warp < 12) {
         // ================= loaders: keys and values of a tile together ===============================
         constexpr int LT = kTileLoaders;
         const int tid = threadIdx.x - 256;
@@ -536,73 +558,89 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         settle(depth - 1);
                     }
                 }
-                attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             settle(0);
         } else {
-            // 16 bytes of codes a turn: 16 (Q8_0) or 32 (Q4_0) values, two or four chunks.  A job, the keys and values
-            // of a tile (of D = 256, Q8_0: either), is fetched while the job before is widened, and only after
-            // that one's codes have arrived.
-            constexpr int RB = KvRow<KIND, D>::bytes, CH = RB / 16, HALF = S::keys * CH;
-            constexpr int jobs = CH > 8 ? 2 : 1, ALL = 2 * HALF / jobs, N = (ALL + LT - 1) / LT;
+            // 16 bytes of codes a turn: 16 (Q8_0) or 32 (Q4_0) values, two or four chunks; a thread has one chunk of R
+            // keys, 128 / CH apart.  Pages of 16 keys and more come through raw buffers that warp 13 fills by bulk copies:
+            // beside 200 KB of shared memory L1 is too small to have many plain loads on their way (they took 1.5 us a
+            // tile, more than the softmax).
+            constexpr int RB = S::rb, CH = RB / 16, R = S::keys * CH / LT, STEP = LT / CH;
+            constexpr int jobs = S::jobs, N = 2 * R / jobs;
             constexpr int OUT = KIND == kKvQ8_0 ? 2 : 4, VALS = 8 * OUT;
+            // eight lanes store two rows of four chunks where rows have them: distinct banks
+            const int in = tid % (2 * CH);
+            const int ch = CH >= 8 ? (in & 3) | ((in >> 3) << 2) : tid % CH;
+            const int r0 = CH >= 8 ? tid / (2 * CH) * 2 + ((in >> 2) & 1) : tid / CH;
+            const bool bulk = c.page_shift >= kTileBulkShift;
             uint4 w[N], wn[N];
-            uint32_t d[N], dn[N], gone = 0;  // gone: bits of the fetched chunks whose key is not there
-            int pages[N], own = 0;           // pages of the next fetch's keys, and of key `tid`
-            // the i-th chunk of this thread: (keys or values, key, chunk); eight lanes store two rows of four
-            // chunks where rows have them: distinct banks
-            auto item = [&](int i, int job, int &kv, int &r, int &ch) {
-                const int at = min(tid + i * LT, ALL - 1) + job * ALL, j = at % HALF, in = j % (2 * CH);
-                kv = at / HALF;
-                ch = CH >= 8 ? (in & 3) | ((in >> 3) << 2) : j % CH;
-                r = CH >= 8 ? j / (2 * CH) * 2 + ((in >> 2) & 1) : j / CH;
-                return tid + i * LT < ALL;
+            uint32_t d[N], dn[N], gone = 0;  // gone: bits of the fetched keys that are not there
+            int pages[R];                    // pages of the next fetch's keys
+            uint32_t taken = 0;              // jobs taken from the raw buffers
+            auto look = [&](const TileUnit<KIND, D> &u, int t) {
+#pragma unroll
+                for (int i = 0; i < R; ++i) pages[i] = page_of(u, t * S::keys + r0 + i * STEP);
+            };
+            constexpr uint32_t flip = KIND == kKvQ8_0 ? 0x80808080u : 0;
+            // a job's codes from the raw buffer that warp 13 had filled
+            auto from_raw = [&](const TileUnit<KIND, D> &u, int t) {
+                const int slot = taken % S::nraw;
+                tile_wait(&sh, &sh.raw_full[slot], (taken / S::nraw) & 1, limit_ns);
+                __syncwarp();
+                const uint8_t *raw = sraw + slot * S::raw;
+                const int left = u.key_end - t * S::keys;
+                const uint32_t bad[2] = {sh.bad[seq & 7][0], sh.bad[seq & 7][1]};
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int r = r0 + i % R * STEP, v = i / R;
+                    const uint4 x = *reinterpret_cast<const uint4 *>(raw + (v * S::keys + r) * RB + ch * 16);
+                    const uint32_t y = *reinterpret_cast<const uint16_t *>(raw + N / R * S::keys * RB + (v * S::keys + r) * S::sb + ch * VALS / 32 * 2);
+                    w[i] = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+                    d[i] = r >= left || ((bad[r >> 5] >> (r & 31)) & 1) ? 0 : dup16(y);
+                }
             };
             // Loads without a condition (of the pool's first row where there is none): loads in branches would be
             // waited for one after the other.
-            auto look = [&](const TileUnit<KIND, D> &u, int t, int job) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    int kv, r, ch;
-                    item(i, job, kv, r, ch);
-                    pages[i] = page_of(u, t * S::keys + r);
-                }
-                if (job == 0) own = page_of(u, t * S::keys + tid);
-            };
             auto fetch = [&](const TileUnit<KIND, D> &u, int t, int job) {
+                const uint8_t *pk = job ? c.v : c.k, *pv = c.v;
+                const uint8_t *sk = reinterpret_cast<const uint8_t *>(job ? c.vs : c.ks), *sv = reinterpret_cast<const uint8_t *>(c.vs);
+                const int co = ch * 16, so = ch * VALS / 32 * 2;
+                auto get = [&](int i, int64_t row) {
+                    wn[i] = ld_stream(pk + row * RB + co);
+                    dn[i] = ld_stream16(sk + row * (D / 16) + so);
+                    if constexpr (jobs == 1) {
+                        wn[R + i] = ld_stream(pv + row * RB + co);
+                        dn[R + i] = ld_stream16(sv + row * (D / 16) + so);
+                    }
+                };
                 gone = 0;
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    int kv, r, ch;
-                    item(i, job, kv, r, ch);
-                    const int64_t rw = row_of(u, t * S::keys + r, pages[i]);
-                    gone |= rw < 0 ? 1u << i : 0;
-                    const int64_t row = max(rw, int64_t(0));
-                    wn[i] = __ldg(reinterpret_cast<const uint4 *>((kv ? c.v : c.k) + row * RB + ch * 16));
-                    dn[i] = __ldg(reinterpret_cast<const unsigned short *>(kv ? c.vs : c.ks) + row * (D / 32) + ch * VALS / 32);
+                for (int i = 0; i < R; ++i) {
+                    const int64_t row = row_of(u, t * S::keys + r0 + i * STEP, pages[i]);
+                    gone |= row < 0 ? 1u << i : 0;
+                    get(i, max(row, int64_t(0)));
                 }
             };
             auto take = [&]() {  // the fetched codes, that is, waits for them
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    constexpr uint32_t flip = KIND == kKvQ8_0 ? 0x80808080u : 0;
                     w[i] = make_uint4(wn[i].x ^ flip, wn[i].y ^ flip, wn[i].z ^ flip, wn[i].w ^ flip);
-                    d[i] = (gone >> i) & 1 ? 0 : dup16(dn[i]);
+                    d[i] = (gone >> (i % R)) & 1 ? 0 : dup16(dn[i]);
                 }
             };
             auto widen = [&](int job, bool check) {
                 const int b = seq % S::nbuf;
                 if (seq >= S::nbuf) {
                     const uint32_t parity = (seq / S::nbuf - 1) & 1;
-                    if (jobs == 1 || job == 0) tile_wait(&sh, &sh.empty[0][b], parity, limit_ns);
-                    if (jobs == 1 || job == 1) tile_wait(&sh, &sh.empty[1][b], parity, limit_ns);
+                    // (a tile's keys are free before its values)
+                    tile_wait(&sh, &sh.empty[jobs == 1 || job == 1][b], parity, limit_ns);
                 }
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    int kv, r, ch;
-                    if (!item(i, job, kv, r, ch)) break;
+                    const int kv = jobs == 1 ? i / R : job, r = r0 + i % R * STEP;
                     uint32_t d2 = d[i];
                     if (check && kv && nonfinite2<false>(d2)) {
                         d2 = 0;
@@ -634,33 +672,42 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             while (p.b < bt.batch && p.unit0 < hi) {
                 const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
                 ++unit;
-                look(u, u.t0, 0);
-                fetch(u, u.t0, 0);
-                int mine = own;  // page of key `tid` of tile t
-                look(u, jobs == 2 ? u.t0 : u.t0 + 1, jobs - 1);
-                for (int t = u.t0; t < u.t1; ++t) {
-                    const bool check = (t + 1) * S::keys > u.free_end, more = t + 1 < u.t1;
-                    share_bad(tid < S::keys && row_of(u, t * S::keys + tid, mine) == -1);
-                    take();
-                    if (jobs == 2) {
-                        fetch(u, t, 1);
-                        look(u, t + 1, 0);
-                        widen(0, false);
+                if (bulk) {
+                    for (int t = u.t0; t < u.t1; ++t, ++seq)
+                        for (int job = 0; job < jobs; ++job, ++taken) {
+                            from_raw(u, t);
+                            widen(job, job == jobs - 1 && (t + 1) * S::keys > u.free_end);
+                            if (lane == 0) mbar_arrive(&sh.raw_empty[taken % S::nraw]);
+                        }
+                } else {
+                    // pages of a few keys: every thread fetches its own, a job ahead of the widening
+                    look(u, u.t0);
+                    fetch(u, u.t0, 0);
+                    int page = page_of(u, u.t0 * S::keys + tid);  // of key `tid` of the tile
+                    if (jobs == 1) look(u, u.t0 + 1);
+                    for (int t = u.t0; t < u.t1; ++t, ++seq) {
+                        const bool check = (t + 1) * S::keys > u.free_end, more = t + 1 < u.t1;
+                        share_bad(tid < S::keys && row_of(u, t * S::keys + tid, page) == -1);
+                        if (tid < S::keys) page = page_of(u, (t + 1) * S::keys + tid);
                         take();
+                        if (jobs == 2) {
+                            fetch(u, t, 1);
+                            look(u, t + 1);
+                            widen(0, false);
+                            take();
+                        }
+                        if (more) {
+                            fetch(u, t + 1, 0);
+                            if (jobs == 1) look(u, t + 2);
+                        }
+                        widen(jobs - 1, check);
                     }
-                    mine = own;
-                    if (more) {
-                        fetch(u, t + 1, 0);
-                        look(u, jobs == 2 ? t + 1 : t + 2, jobs - 1);
-                    }
-                    widen(jobs - 1, check);
-                    ++seq;
                 }
-                attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
             }
         }
     } else {
-        if (elect_one()) {
+        if (warp == 12 && elect_one()) {
             // ================= products ================================================================
             constexpr uint32_t fmt = BF ? 1 : 0;
             constexpr uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
@@ -695,41 +742,120 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                 for (int w = 0; w < S::nq; ++w)
                     if (w < active) tile_wait(&sh, &sh.q_full[w], nq[w]++ & 1, limit_ns);
-                // One tile ahead of the softmax: S of tile i + 1 goes to the other turn's columns, whose P was read
-                // by the products of tile i - 1, which were issued before.
-                for (int i = -1; i < tiles; ++i) {
-                    if (i + 1 < tiles) {
-                        const uint32_t b = nb + i + 1;
-                        wait_full(0, b);
+                auto scores = [&](int i, int w) { qk(w, i & 1, (nb + i) % S::nbuf); };
+                auto values = [&](int i, int w) {
+                    if (i & 1) tile_wait(&sh, &sh.p_full[w][1], np[w][1]++ & 1, limit_ns);
+                    else tile_wait(&sh, &sh.p_full[w][0], np[w][0]++ & 1, limit_ns);
+                    fence_after();
+                    pv(w, i & 1, (nb + i) % S::nbuf, i > 0);
+                };
+                if constexpr (S::nq == 2) {
+                    // Two tiles ahead of the softmax: when a row tile's P V of tile i is issued, its columns take the scores
+                    // of tile i + 2, while the softmax works on those of i + 1.  Row tiles do not wait for each other.
+                    for (int i = 0; i < min(tiles, 2); ++i) {
+                        wait_full(0, nb + i);
 #pragma unroll
-                        for (int w = 0; w < S::nq; ++w)
-                            if (w < active) qk(w, (i + 1) & 1, b % S::nbuf);
-                        mma_commit(&sh.empty[0][b % S::nbuf]);
+                        for (int w = 0; w < 2; ++w)
+                            if (w < active) scores(i, w);
+                        mma_commit(&sh.empty[0][(nb + i) % S::nbuf]);
                     }
-                    if (i < 0) continue;
-                    const uint32_t b = nb + i;
-                    wait_full(1, b);
+                    for (int i = 0; i < tiles; ++i) {
+                        const bool more = i + 2 < tiles;
 #pragma unroll
-                    for (int w = 0; w < S::nq; ++w)
-                        if (w < active) {
-                            if (i & 1) tile_wait(&sh, &sh.p_full[w][1], np[w][1]++ & 1, limit_ns);
-                            else tile_wait(&sh, &sh.p_full[w][0], np[w][0]++ & 1, limit_ns);
-                            fence_after();
-                            pv(w, i & 1, b % S::nbuf, i > 0);
+                        for (int w = 0; w < 2; ++w)
+                            if (w < active) {
+                                if (w == 0) wait_full(1, nb + i);
+                                values(i, w);
+                                if (more) {
+                                    if (w == 0) wait_full(0, nb + i + 2);
+                                    scores(i + 2, w);
+                                }
+                            }
+                        mma_commit(&sh.empty[1][(nb + i) % S::nbuf]);
+                        if (more) mma_commit(&sh.empty[0][(nb + i + 2) % S::nbuf]);
+                    }
+                } else {
+                    // One tile ahead (two buffers of each kind): S of tile i + 1 goes to the other turn's columns, whose P
+                    // was read by the products of tile i - 1, which were issued before.
+                    for (int i = -1; i < tiles; ++i) {
+                        if (i + 1 < tiles) {
+                            wait_full(0, nb + i + 1);
+                            scores(i + 1, 0);
+                            mma_commit(&sh.empty[0][(nb + i + 1) % S::nbuf]);
                         }
-                    mma_commit(&sh.empty[1][b % S::nbuf]);
+                        if (i < 0) continue;
+                        wait_full(1, nb + i);
+                        values(i, 0);
+                        mma_commit(&sh.empty[1][(nb + i) % S::nbuf]);
+                    }
                 }
                 nb += tiles;
-                attn_next<S::rows, S::keys, kTileCost>(c, bt, p, u.q);
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
             }
             mma_commit(&sh.drain);
             tile_wait(&sh, &sh.drain, 0, limit_ns);
+        }
+        if (warp == 13 && S::quant && c.page_shift >= kTileBulkShift) {
+            // ================= raw buffers: bulk copies, page by page ====================================
+            const int per = min(S::keys, 1 << c.page_shift), parts = S::keys / per;  // keys of a copy, copies of a tile
+            uint32_t filled = 0;
+            int seq = 0;
+            while (p.b < bt.batch && p.unit0 < hi) {
+                const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                auto page_of = [&](int t) {  // lane i: the page of part i
+                    const int key = t * S::keys + lane * per;
+                    return lane < parts && key < u.key_end ? __ldg(bt.table + p.b * bt.table_stride + (key >> c.page_shift)) : -1;
+                };
+                int page = page_of(u.t0);
+                for (int t = u.t0; t < u.t1; ++t, ++seq) {
+                    const int key = t * S::keys + lane * per;
+                    const bool here = lane < parts && key < u.key_end;
+                    const int64_t row = here ? kv_row(page, c.num_pages, p.head, c.kv_heads, key & ((1 << c.page_shift) - 1), c.page_shift) : -1;
+                    page = page_of(t + 1);
+                    const uint32_t live = __ballot_sync(0xffffffffu, row >= 0), none = __ballot_sync(0xffffffffu, here && row < 0);
+                    for (int job = 0; job < S::jobs; ++job, ++filled) {
+                        const int slot = filled % S::nraw;
+                        if (filled >= S::nraw) tile_wait(&sh, &sh.raw_empty[slot], (filled / S::nraw - 1) & 1, limit_ns);
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (job == 0) {
+                                uint64_t bad = 0;
+                                for (int i = 0; i < parts; ++i)
+                                    if ((none >> i) & 1) bad |= (per == 64 ? ~uint64_t(0) : (uint64_t(1) << per) - 1) << (i * per);
+                                sh.bad[seq & 7][0] = uint32_t(bad);
+                                sh.bad[seq & 7][1] = uint32_t(bad >> 32);
+                                if (bad) flag_bad_page();
+                            }
+                            mbar_arrive_expect_tx(&sh.raw_full[slot], __popc(live) * per * (S::rb + S::sb) * 2 / S::jobs);
+                        }
+                        __syncwarp();
+                        uint8_t *raw = sraw + slot * S::raw;
+                        for (int i = 0; i < parts; ++i) {
+                            const int64_t first = __shfl_sync(0xffffffffu, row, i);
+                            if (first >= 0 && elect_one()) {
+#pragma unroll
+                                for (int v = 0; v < 2 / S::jobs; ++v) {
+                                    const bool values = S::jobs == 2 ? job == 1 : v == 1;
+                                    bulk_copy_g2s(raw + (v * S::keys + i * per) * S::rb, (values ? c.v : c.k) + first * S::rb,
+                                                  per * S::rb, &sh.raw_full[slot]);
+                                    bulk_copy_g2s(raw + 2 / S::jobs * S::keys * S::rb + (v * S::keys + i * per) * S::sb,
+                                                  reinterpret_cast<const uint8_t *>(values ? c.vs : c.ks) + first * S::sb, per * S::sb,
+                                                  &sh.raw_full[slot]);
+                                }
+                            }
+                            __syncwarp();
+                        }
+                    }
+                }
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
+            }
+            // (every copy has landed before the loaders, and so the CTA, are done)
         }
         __syncwarp();
     }
     fence_before();
     __syncthreads();
-    if (warp == 15) {
+    if (warp == 12) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
