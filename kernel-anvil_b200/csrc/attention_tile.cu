@@ -115,7 +115,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
 
 struct TileShared {
     AttnScratch sc;
-    uint64_t full[2][4], empty[2][4], raw_full[3], raw_empty[3], q_full[2],  // [keys, values][buffer]
+    uint64_t full[2][4], empty[2][4], raw_full[3], raw_empty[3], partial, q_full[2],  // [keys, values][buffer]
          s_full[2][2], p_full[2][2], pv_done[2][2], drain;  // [row tile][turn]
     uint32_t tmem;
     int failed;             // a wait gave up: later ones do not wait
@@ -140,6 +140,7 @@ __device__ __forceinline__ void tile_wait(TileShared *sh, uint64_t *bar, uint32_
         }
     }
 }
+__device__ __forceinline__ void loaders_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kTileLoaders) : "memory"); }
 // Whether a phase is over, without the wait that try_wait may take.
 __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
     uint32_t ok;
@@ -223,6 +224,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 mbar_init(&sh.pv_done[i][x], 1);
             }
         }
+        mbar_init(&sh.partial, 1);
         mbar_init(&sh.drain, 1);
         mbar_fence_init();
         sh.failed = 0;
@@ -460,108 +462,145 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             return sbuf + (kv * S::nbuf + b) * S::buf + (oc >> 3) * (S::keys * 128) + r * 128 + (((oc & 7) ^ (r & 7)) << 4);
         };
         if constexpr (!S::quant) {
-            // 16-bit rows go straight to their places.  A tile that every row sees whole, in pages of 8 keys and more,
-            // is copied by TMA, a box of up to 64 keys of one page and 64 columns at a time; others by cp.async, whose
-            // tiles are announced when the next one's copies are on their way.
-            constexpr int CH = D / 8, ALL = 2 * S::keys * CH, depth = S::nbuf > 2 ? 2 : 1;
-            const int boxes = box ? S::keys / box : 0;  // of a tile's keys; box 0: no TMA
-            int pending = 0;
-            auto settle = [&](int left) {  // announces all but the newest `left` tiles, whose copies are done
-                for (; pending > left; --pending) {
-                    const int b = (seq - pending) % S::nbuf;
-                    announce(0, b);
-                    if (lane == 0) mbar_arrive(&sh.full[1][b]);
+            // 16-bit rows go straight to their places: from pages of 8 keys and more by TMA, boxes of up to 64 keys of one
+            // page and 64 columns; from smaller ones by cp.async, a tile announced when the next one's copies are on their way.
+            // Of a tile that some row does not see whole, or that lacks pages, what is not finite and what is no key
+            // leaves the values first (see the outputs).
+            constexpr int CH = D / 8;
+            auto clean = [&](const TileUnit<KIND, D> &u, int t, int b) {
+                const int left = u.key_end - t * S::keys;
+                const uint32_t bad[2] = {sh.bad[seq & 7][0], sh.bad[seq & 7][1]};
+#pragma unroll 2
+                for (int at = tid; at < S::keys * CH; at += LT) {
+                    const int r = at / CH;
+                    uint4 *w4 = reinterpret_cast<uint4 *>(place(1, b, r, at % CH));
+                    const uint4 x = *w4;
+                    const uint32_t n[4] = {nonfinite2<BF>(x.x), nonfinite2<BF>(x.y), nonfinite2<BF>(x.z), nonfinite2<BF>(x.w)};
+                    if (r >= left || ((bad[r >> 5] >> (r & 31)) & 1)) {
+                        *w4 = make_uint4(0, 0, 0, 0);
+                    } else if (n[0] | n[1] | n[2] | n[3]) {
+                        *w4 = make_uint4(x.x & ~n[0], x.y & ~n[1], x.z & ~n[2], x.w & ~n[3]);
+                        *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
+                    }
                 }
+                __syncwarp();
             };
-            while (p.b < bt.batch && p.unit0 < hi) {
-                const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
-                ++unit;
-                // lane i: the page of box i
-                int page = lane < boxes ? page_of(u, u.t0 * S::keys + lane * box) : 0;
-                for (int t = u.t0; t < u.t1; ++t) {
-                    const bool check = (t + 1) * S::keys > u.free_end;
-                    const int64_t row = lane < boxes ? row_of(u, t * S::keys + lane * box, page) : 0;
-                    const bool fast = boxes && !check && !__any_sync(0xffffffffu, row < 0);
-                    if (lane < boxes && t + 1 < u.t1) page = page_of(u, (t + 1) * S::keys + lane * box);
-                    const int b = seq % S::nbuf;
-                    const uint32_t parity = (seq / S::nbuf - 1) & 1;
-                    // (a product may wait for a pending tile before it frees this one's buffers)
-                    if (pending && (fast || !__all_sync(0xffffffffu, seq < S::nbuf || mbar_test(&sh.empty[1][b], parity)))) {
-                        asm volatile("cp.async.wait_group 0;" ::: "memory");
-                        settle(0);
-                    }
-                    if (seq >= S::nbuf) {
-                        tile_wait(&sh, &sh.empty[0][b], parity, limit_ns);
-                        tile_wait(&sh, &sh.empty[1][b], parity, limit_ns);
-                        __syncwarp();
-                    }
-                    if (fast) {
-                        share_bad(false);
+            auto announce_both = [&](int b) {
+                announce(0, b);
+                if (lane == 0) mbar_arrive(&sh.full[1][b]);
+            };
+            auto wait_empty = [&](int b, uint32_t parity) {
+                tile_wait(&sh, &sh.empty[1][b], parity, limit_ns);  // (a tile's keys are free before its values)
+                __syncwarp();
+            };
+            if (box) {
+                const int boxes = S::keys / box;  // of a tile's keys
+                uint32_t partial = 0;             // tiles that were cleaned
+                while (p.b < bt.batch && p.unit0 < hi) {
+                    const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                    ++unit;
+                    // lane i: the page of box i
+                    int page = lane < boxes ? page_of(u, u.t0 * S::keys + lane * box) : 0;
+                    for (int t = u.t0; t < u.t1; ++t, ++seq) {
+                        const int64_t row = lane < boxes ? row_of(u, t * S::keys + lane * box, page) : -2;
+                        if (lane < boxes && t + 1 < u.t1) page = page_of(u, (t + 1) * S::keys + lane * box);
+                        const uint32_t live = __ballot_sync(0xffffffffu, row >= 0), none = __ballot_sync(0xffffffffu, row == -1);
+                        const bool fast = (t + 1) * S::keys <= u.free_end && !none;
+                        const int b = seq % S::nbuf;
+                        if (seq >= S::nbuf) wait_empty(b, (seq / S::nbuf - 1) & 1);
                         if (warp == 8) {
+                            uint64_t *bk = fast ? &sh.full[0][b] : &sh.partial, *bv = fast ? &sh.full[1][b] : &sh.partial;
+                            if (lane == 0) {
+                                uint64_t bad = 0;
+                                for (int i = 0; i < boxes; ++i)
+                                    if ((none >> i) & 1) bad |= (box == 64 ? ~uint64_t(0) : (uint64_t(1) << box) - 1) << (i * box);
+                                sh.bad[seq & 7][0] = uint32_t(bad);
+                                sh.bad[seq & 7][1] = uint32_t(bad >> 32);
+                                if (bad) flag_bad_page();
+                                const int bytes = __popc(live) * box * D * 2;
+                                if (fast) {
+                                    mbar_arrive_expect_tx(bk, bytes);
+                                    mbar_arrive_expect_tx(bv, bytes);
+                                } else {
+                                    mbar_arrive_expect_tx(bk, 2 * bytes);
+                                }
+                            }
                             __syncwarp();
                             for (int i = 0; i < boxes; ++i) {
                                 const int y = int(__shfl_sync(0xffffffffu, row, i));
-                                if (elect_one()) {
-                                    if (i == 0) {
-                                        mbar_arrive_expect_tx(&sh.full[0][b], S::buf);
-                                        mbar_arrive_expect_tx(&sh.full[1][b], S::buf);
-                                    }
+                                if (y >= 0 && elect_one()) {
 #pragma unroll
                                     for (int j = 0; j < S::blocks; ++j) {
-                                        tma_box(place(0, b, i * box, 8 * j), &map_k, 64 * j, y, &sh.full[0][b]);
-                                        tma_box(place(1, b, i * box, 8 * j), &map_v, 64 * j, y, &sh.full[1][b]);
+                                        tma_box(place(0, b, i * box, 8 * j), &map_k, 64 * j, y, bk);
+                                        tma_box(place(1, b, i * box, 8 * j), &map_v, 64 * j, y, bv);
                                     }
                                 }
                                 __syncwarp();
                             }
-                        } else if (lane == 0) {
+                        } else if (fast && lane == 0) {
                             mbar_arrive(&sh.full[0][b]);
                             mbar_arrive(&sh.full[1][b]);
                         }
-                        ++seq;
-                        continue;
+                        if (!fast) {
+                            tile_wait(&sh, &sh.partial, partial++ & 1, limit_ns);
+                            loaders_sync();  // nobody arms it again before all have seen this phase
+                            clean(u, t, b);
+                            announce_both(b);
+                        }
                     }
-                    {
+                    attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
+                }
+            } else {
+                constexpr int ALL = 2 * S::keys * CH, depth = S::nbuf > 2 ? 2 : 1;
+                int pending = 0;
+                auto settle = [&](int left) {  // announces all but the newest `left` tiles, whose copies are done
+                    for (; pending > left; --pending) announce_both((seq - pending) % S::nbuf);
+                };
+                while (p.b < bt.batch && p.unit0 < hi) {
+                    const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                    ++unit;
+                    for (int t = u.t0; t < u.t1; ++t) {
+                        const int b = seq % S::nbuf;
+                        if (seq >= S::nbuf) {
+                            const uint32_t parity = (seq / S::nbuf - 1) & 1;
+                            // (a product may wait for a pending tile before it frees this one's buffers)
+                            if (pending && !__all_sync(0xffffffffu, mbar_test(&sh.empty[1][b], parity))) {
+                                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                                settle(0);
+                            }
+                            wait_empty(b, parity);
+                        }
                         const int key = t * S::keys + tid;
                         share_bad(tid < S::keys && row_of(u, key, page_of(u, key)) == -1);
-                    }
-#pragma unroll
-                    for (int i = 0; i < (ALL + LT - 1) / LT; ++i) {
-                        const int at = tid + i * LT, kv = at / (ALL / 2), r = at / CH % S::keys, ch = at % CH;
-                        if (at >= ALL) break;
-                        const int64_t rw = row_of(u, t * S::keys + r, page_of(u, t * S::keys + r));
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(place(kv, b, r, ch))),
-                                     "l"((kv ? c.v : c.k) + max(rw, int64_t(0)) * (2 * D) + ch * 16), "r"(rw < 0 ? 0 : 16)
-                                     : "memory");
-                    }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    ++seq;
-                    ++pending;
-                    if (check) {
-                        // a masked tile's values: what is not finite leaves the product (see the outputs)
-                        asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll 1
+#pragma unroll 8
                         for (int at = tid; at < ALL; at += LT) {
-                            if (at < ALL / 2) continue;
-                            uint4 *w4 = reinterpret_cast<uint4 *>(place(1, b, at / CH % S::keys, at % CH));
-                            const uint4 x = *w4;
-                            const uint32_t n[4] = {nonfinite2<BF>(x.x), nonfinite2<BF>(x.y), nonfinite2<BF>(x.z), nonfinite2<BF>(x.w)};
-                            if (n[0] | n[1] | n[2] | n[3]) {
-                                *w4 = make_uint4(x.x & ~n[0], x.y & ~n[1], x.z & ~n[2], x.w & ~n[3]);
-                                *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
+                            const int kv = at / (ALL / 2), r = at / CH % S::keys, ch = at % CH;
+                            const int64_t rw = row_of(u, t * S::keys + r, page_of(u, t * S::keys + r));
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(place(kv, b, r, ch))),
+                                         "l"((kv ? c.v : c.k) + max(rw, int64_t(0)) * (2 * D) + ch * 16), "r"(rw < 0 ? 0 : 16)
+                                         : "memory");
+                        }
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        if ((t + 1) * S::keys > u.free_end) {
+                            asm volatile("cp.async.wait_group 0;" ::: "memory");
+                            settle(0);
+                            loaders_sync();  // a thread cleans what others copied, by the mask that others wrote
+                            clean(u, t, b);
+                            announce_both(b);
+                            ++seq;
+                        } else {
+                            ++seq;
+                            if (++pending == depth) {
+                                asm volatile("cp.async.wait_group %0;" ::"n"(depth - 1) : "memory");
+                                settle(depth - 1);
                             }
                         }
-                        __syncwarp();
-                        settle(0);
-                    } else if (pending == depth) {
-                        asm volatile("cp.async.wait_group %0;" ::"n"(depth - 1) : "memory");
-                        settle(depth - 1);
                     }
+                    attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
                 }
-                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                settle(0);
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            settle(0);
         } else {
             // 16 bytes of codes a turn: 16 (Q8_0) or 32 (Q4_0) values, two or four chunks; a thread has one chunk of R
             // keys, 128 / CH apart.  Pages of 16 keys and more come through raw buffers that warp 13 fills by bulk copies:
