@@ -11,12 +11,15 @@
 // keys fill tensor memory with one turn, P over S: the chain softmax, P V, Q K^T, softmax then left
 // both sides idle half of the time: 2.68 against FILLCHUNK ms for 2048 rows over 30049 keys.)
 // Warp roles: warps 0-3 and 4-7 are the softmax of the two row tiles; warps 8-11 bring keys and values
-// through the page table into rings of buffers in the 128-byte swizzled layout, widening quantised
-// codes to fp16 on the way; warp 12 issues every product.  All hand-over is by mbarriers; each wait is bounded and
-// a failure makes the later ones return at once.
+// through the page table into a ring of buffers in the 128-byte swizzled layout, widening quantised
+// codes to fp16 on the way, and a unit's queries while the softmax is at the unit before; warps 12 and 13
+// issue the products of a row tile each (one warp for both took 1900 cycles a tile to issue and
+// hand over, more than the products took); warp 14 fetches quantised codes.  All hand-over is by mbarriers;
+// each wait is bounded and a failure makes the later ones return at once.
 //
-// The running maximum is only raised when it grew by more than 2^8 (weights may then reach 2^8, which
-// fp16 and fp32 hold without loss), so that O is rescaled a few times a row instead of at every tile.
+// Weights are taken by a reference, the maximum of a row's first tile; it is raised, and O rescaled, only when
+// a tile's weights sum to more than 2^15 (fp16 and fp32 hold them without loss), which the sum that
+// is taken anyway shows: most tiles are never searched for their maximum.
 #include <cuda.h>
 
 #include <algorithm>
@@ -31,7 +34,7 @@ constexpr int kTileThreads = 512;   // 128 registers a thread at launch, divided
 constexpr int kTileLoaders = 128;   // threads of the four loading warps
 constexpr int kTileCost = 8;        // beginning and ending a unit, in key tiles
 constexpr int kTileBulkShift = 4;   // pages of 16 keys: their scales are whole 16-byte pieces
-constexpr float kTileSlack = 8.0f;  // log2 of how far weights may exceed 1
+constexpr float kTileSlack = 32768.0f;  // the largest sum of a tile's weights, and so weight
 
 template <int KIND, int D> struct TileShape {
     static constexpr int nq = D == 256 ? 1 : 2;         // row tiles of 128
@@ -43,8 +46,10 @@ template <int KIND, int D> struct TileShape {
     static constexpr bool bf16 = KIND == kKvBF16;
     static constexpr bool quant = KIND == kKvQ8_0 || KIND == kKvQ4_0;
     static constexpr int nbuf = D == 256 ? 2 : D == 128 && quant ? 3 : 4;  // buffers of keys, and of values
-    // quantised: a tile's codes and scales as they are in the cache, keys and values together (D = 256: a job each)
+    // A tile's keys and values are loaded and freed together where there are buffers for more than two tiles; else
+    // they are a job each, so that the next keys come while the last values are in use.
     static constexpr int jobs = D == 256 ? 2 : 1;
+    // quantised: a job's codes and scales as they are in the cache
     static constexpr int rb = KvRow<KIND, D>::bytes, sb = KvRow<KIND, D>::scales * 2;
     static constexpr int raw = quant ? keys * (rb + sb) * 2 / jobs : 0;
     static constexpr int nraw = D == 256 && KIND == kKvQ8_0 ? 1 : 3;
@@ -103,6 +108,10 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *v) {
                  "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::W8(v, 0), W8(v, 8), W8(v, 16), W8(v, 24), "r"(addr)
                  : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t *v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : R8(v, 0), R8(v, 8) : "r"(addr));
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::W8(v, 0),
                  W8(v, 8), "r"(addr)
@@ -115,8 +124,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
 
 struct TileShared {
     AttnScratch sc;
-    uint64_t full[2][4], empty[2][4], raw_full[3], raw_empty[3], partial, q_full[2],  // [keys, values][buffer]
-         s_full[2][2], p_full[2][2], pv_done[2][2], drain;  // [row tile][turn]
+    uint64_t full[2][4], empty[2][4], raw_full[3], raw_empty[3], partial, q_full, q_free,  // [job][buffer]
+         s_full[2][2], p_full[2][2], pv_done[2][2], drain[2];  // [row tile][turn]
+    float fac[2][256];      // [unit % 2]: what a row's scores are multiplied by
     uint32_t tmem;
     int failed;             // a wait gave up: later ones do not wait
     int dirty[8];           // [unit % 8] = unit where non-finite values were taken out of its value tiles
@@ -210,14 +220,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int i = 0; i < S::nbuf; ++i)
             for (int kv = 0; kv < 2; ++kv) {
                 mbar_init(&sh.full[kv][i], kTileLoaders / 32);
-                mbar_init(&sh.empty[kv][i], 1);
+                mbar_init(&sh.empty[kv][i], S::nq);
             }
         for (int i = 0; i < S::nraw; ++i) {
             mbar_init(&sh.raw_full[i], 1);
             mbar_init(&sh.raw_empty[i], kTileLoaders / 32);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.q_full[i], 4);
             for (int x = 0; x < 2; ++x) {
                 mbar_init(&sh.s_full[i][x], 1);
                 mbar_init(&sh.p_full[i][x], 4);
@@ -225,7 +234,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
         }
         mbar_init(&sh.partial, 1);
-        mbar_init(&sh.drain, 1);
+        mbar_init(&sh.q_full, kTileLoaders / 32);
+        mbar_init(&sh.q_free, S::nq);
+        for (int i = 0; i < 2; ++i) mbar_init(&sh.drain[i], 1);
         mbar_fence_init();
         sh.failed = 0;
         for (int i = 0; i < 8; ++i) sh.dirty[i] = 0;
@@ -256,52 +267,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
                 ++unit;
                 if (w * 128 < u.nrows) {
-                    // ---- this row's query, into the swizzled operand
                     const int ur = w * 128 + r;
                     const bool live = ur < u.nrows;
                     const unsigned rr = unsigned(p.mt) * S::rows + ur;
                     const int tok = int(rr / unsigned(u.q.group)), h = p.head * u.q.group + int(rr - unsigned(tok) * u.q.group);
                     const int seen = live ? min(u.key_end, kv_seen(tok, u.q.n, u.q.s.kv, u.q.causal)) : 0;
-                    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(io.q) +
-                                                                       (u.q.s.q0 + int64_t(tok)) * io.q_row + h * io.q_head);
-                    int ex = 0;
-                    if (S::quant && io.q_bf16 && live) {
-                        uint32_t m = 0;
-#pragma unroll 8
-                        for (int i = 0; i < D / 8; ++i) {
-                            const uint4 x = __ldg(src + i);
-                            const uint32_t y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) m = max(max(m, y[j] & 0x7FFFu), (y[j] >> 16) & 0x7FFFu);
-                        }
-                        ex = q_exponent(m << 16);
-                    }
-                    const float up = pow2i(ex);
-                    uint8_t *dq = sq + w * 128 * 128 + r * 128;
-#pragma unroll 8
-                    for (int i = 0; i < D / 8; ++i) {
-                        uint4 x = live ? __ldg(src + i) : make_uint4(0, 0, 0, 0);
-                        if (S::quant && io.q_bf16) {
-                            uint32_t y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                y[j] = pack_half(__uint_as_float(y[j] << 16) * up, __uint_as_float(y[j] & 0xFFFF0000u) * up);
-                            x = make_uint4(y[0], y[1], y[2], y[3]);
-                        }
-                        if (io.scale_log2 < 0.0f) {  // a negative scale: -q, so that the largest score stays the largest
-                            x.x ^= 0x80008000u;
-                            x.y ^= 0x80008000u;
-                            x.z ^= 0x80008000u;
-                            x.w ^= 0x80008000u;
-                        }
-                        *reinterpret_cast<uint4 *>(dq + (i >> 3) * (S::rows * 128) + (((i & 7) ^ (r & 7)) << 4)) = x;
-                    }
-                    // (above zero, so that a masked score stays -inf)
-                    const float fac = fmaxf(fabsf(io.scale_log2) * pow2i(-ex), 1e-36f);
-                    fence_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.q_full[w]);
-
+                    float fac = 0.0f;
                     float m = -INFINITY, l = 0.0f;
                     const uint32_t to = tmem + lanes + S::o_col + w * S::o_cols;
                     for (int t = u.t0; t < u.t1; ++t) {
@@ -310,6 +281,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         tile_wait(&sh, &sh.s_full[w][x], (x ? n1 : n0) & 1, limit_ns);
                         __syncwarp();
                         fence_after();
+                        if (t == u.t0) fac = sh.fac[unit & 1][ur];  // written with the query
                         uint32_t s[64];
                         tmem_ld32(ts, s);
                         tmem_ld32(ts + 32, s + 32);
@@ -321,48 +293,58 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             for (int i = 0; i < 64; ++i)
                                 if (i >= left || ((bad[i >> 5] >> (i & 31)) & 1)) s[i] = 0xFF800000u;
                         }
-                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        // The weights of this tile by the row's reference m so far; only where their sum shows one beyond
+                        // 2^15 (fp16 ends at 65504), or where there is no reference yet, is the maximum looked for, made
+                        // the reference, and the tile taken again.
+                        float sum = 0.0f;
+                        uint32_t y[32];
+                        bool raise = m == -INFINITY;
+                        for (int pass = 0;; ++pass) {
+                            if (__any_sync(0xffffffffu, raise)) {
+                                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int i = 0; i < 64; i += 2)
-                            mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac;
-                        const bool raise = mt > m + kTileSlack || (m == -INFINITY && mt > m);
-                        if (__any_sync(0xffffffffu, raise)) {
-                            const float mn = raise ? mt : m;
-                            const float a = raise ? ex2(m - mn) : 1.0f;
-                            if (t > u.t0) {
-                                tile_wait(&sh, &sh.pv_done[w][x ^ 1], ((x ? n0 : n1) - 1) & 1, limit_ns);  // the last tile's P V
-                                __syncwarp();
-                                fence_after();
+                                for (int i = 0; i < 64; i += 2)
+                                    mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac;
+                                const float mn = raise && mt > m ? mt : m;
+                                const float a = mn > m ? ex2(m - mn) : 1.0f;
+                                if (t > u.t0) {
+                                    tile_wait(&sh, &sh.pv_done[w][x ^ 1], ((x ? n0 : n1) - 1) & 1, limit_ns);  // the last tile's P V
+                                    __syncwarp();
+                                    fence_after();
 #pragma unroll 1
-                                for (int i = 0; i < D / 32; ++i) {
-                                    uint32_t v[32];
-                                    tmem_ld32(to + 32 * i, v);
-                                    wait_ld();
+                                    for (int i = 0; i < D / 16; ++i) {
+                                        uint32_t v[16];
+                                        tmem_ld16(to + 16 * i, v);
+                                        wait_ld();
 #pragma unroll
-                                    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * a);
-                                    tmem_st32(to + 32 * i, v);
+                                        for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * a);
+                                        tmem_st16(to + 16 * i, v);
+                                    }
                                 }
+                                l *= a;
+                                m = mn;
                             }
-                            l *= a;
-                            m = mn;
-                        }
-                        const float nb = m == -INFINITY ? 0.0f : -m;
-                        const uint64_t fac2 = pack2(fac, fac), nb2 = pack2(nb, nb);
-                        uint64_t sum[2] = {0, 0};
+                            const float nb = m == -INFINITY ? 0.0f : -m;
+                            const uint64_t fac2 = pack2(fac, fac), nb2 = pack2(nb, nb);
+                            uint64_t sums[2] = {0, 0};
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            float e0, e1;
-                            unpack2(fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), fac2, nb2), e0, e1);
-                            e0 = ex2(e0);
-                            e1 = ex2(e1);
-                            sum[i & 1] = add2(sum[i & 1], pack2(e0, e1));
-                            s[i] = BF ? pack_bf16(e0, e1) : pack_half(e0, e1);
+                            for (int i = 0; i < 32; ++i) {
+                                float e0, e1;
+                                unpack2(fma2(pack2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), fac2, nb2), e0, e1);
+                                e0 = ex2(e0);
+                                e1 = ex2(e1);
+                                sums[i & 1] = add2(sums[i & 1], pack2(e0, e1));
+                                y[i] = BF ? pack_bf16(e0, e1) : pack_half(e0, e1);
+                            }
+                            float a0, a1;
+                            unpack2(add2(sums[0], sums[1]), a0, a1);
+                            sum = a0 + a1;
+                            raise = pass == 0 && sum > kTileSlack;
+                            if (!__any_sync(0xffffffffu, raise)) break;
                         }
-                        tmem_st32(ts, s);
-                        float a0, a1;
-                        unpack2(add2(sum[0], sum[1]), a0, a1);
-                        l += a0 + a1;
+                        l += sum;
+                        tmem_st32(ts, y);
                         wait_st();
                         fence_before();
                         __syncwarp();
@@ -434,10 +416,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         constexpr int LT = kTileLoaders;
         const int tid = threadIdx.x - 256;
         int unit = 0, seq = 0;  // units and tiles begun
-        auto announce = [&](int kv, int b) {
+        auto announce = [&](int job, int b) {
             fence_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.full[kv][b]);
+            if (lane == 0) mbar_arrive(&sh.full[job][b]);
         };
         // Page of a key (0 behind the last one), looked up a tile ahead of its use; and the key's cache row, -1 where
         // there is no page and -2 behind the last key.
@@ -456,6 +438,55 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 sh.bad[seq & 7][tid >> 5] = bad;
                 if (bad) flag_bad_page();
             }
+        };
+        // A unit's query rows into the swizzled operand, while the softmax is still at the unit before: once that one's
+        // scores are all taken.  Rows that are none are zeros.
+        auto load_q = [&](const TileUnit<KIND, D> &u) {
+            constexpr int CHQ = D / 8, FLY = 4;
+            if (unit > 1) {
+                tile_wait(&sh, &sh.q_free, unit & 1, limit_ns);
+                __syncwarp();
+            }
+            const int all = (u.nrows > 128 ? S::rows : 128) * CHQ;
+            for (int at0 = tid; at0 < all; at0 += FLY * LT) {
+                uint4 x[FLY];
+#pragma unroll
+                for (int f = 0; f < FLY; ++f) {
+                    const int at = at0 + f * LT, ur = at / CHQ, ch = at % CHQ;
+                    const unsigned rr = unsigned(p.mt) * S::rows + ur;
+                    const int tok = int(rr / unsigned(u.q.group)), h = p.head * u.q.group + int(rr - unsigned(tok) * u.q.group);
+                    x[f] = ur < u.nrows ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(io.q) +
+                                                (u.q.s.q0 + int64_t(tok)) * io.q_row + h * io.q_head) + ch)
+                                        : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int f = 0; f < FLY; ++f) {
+                    const int at = at0 + f * LT, ur = at / CHQ, ch = at % CHQ;
+                    uint32_t y[4] = {x[f].x, x[f].y, x[f].z, x[f].w};
+                    int ex = 0;
+                    if (S::quant && io.q_bf16) {
+                        uint32_t m = 0;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) m = max(max(m, y[j] & 0x7FFFu), (y[j] >> 16) & 0x7FFFu);
+#pragma unroll
+                        for (int o = CHQ / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                        ex = q_exponent(m << 16);
+                        const float up = pow2i(ex);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            y[j] = pack_half(__uint_as_float(y[j] << 16) * up, __uint_as_float(y[j] & 0xFFFF0000u) * up);
+                    }
+                    // a negative scale: -q, so that the largest score stays the largest
+                    const uint32_t sign = io.scale_log2 < 0.0f ? 0x80008000u : 0;
+                    *reinterpret_cast<uint4 *>(sq + (ch >> 3) * (S::rows * 128) + ur * 128 + (((ch & 7) ^ (ur & 7)) << 4)) =
+                        make_uint4(y[0] ^ sign, y[1] ^ sign, y[2] ^ sign, y[3] ^ sign);
+                    // (above zero, so that a masked score stays -inf)
+                    if (ch == 0) sh.fac[unit & 1][ur] = fmaxf(fabsf(io.scale_log2) * pow2i(-ex), 1e-36f);
+                }
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.q_full);
         };
         // place of 16-byte chunk oc of key r in a buffer
         auto place = [&](int kv, int b, int r, int oc) {
@@ -485,12 +516,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 __syncwarp();
             };
-            auto announce_both = [&](int b) {
-                announce(0, b);
-                if (lane == 0) mbar_arrive(&sh.full[1][b]);
-            };
-            auto wait_empty = [&](int b, uint32_t parity) {
-                tile_wait(&sh, &sh.empty[1][b], parity, limit_ns);  // (a tile's keys are free before its values)
+            auto wait_empty = [&](int job, int b) {
+                if (seq >= S::nbuf) tile_wait(&sh, &sh.empty[job][b], (seq / S::nbuf - 1) & 1, limit_ns);
                 __syncwarp();
             };
             if (box) {
@@ -499,53 +526,52 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 while (p.b < bt.batch && p.unit0 < hi) {
                     const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
                     ++unit;
+                    load_q(u);
                     // lane i: the page of box i
                     int page = lane < boxes ? page_of(u, u.t0 * S::keys + lane * box) : 0;
                     for (int t = u.t0; t < u.t1; ++t, ++seq) {
                         const int64_t row = lane < boxes ? row_of(u, t * S::keys + lane * box, page) : -2;
                         if (lane < boxes && t + 1 < u.t1) page = page_of(u, (t + 1) * S::keys + lane * box);
                         const uint32_t live = __ballot_sync(0xffffffffu, row >= 0), none = __ballot_sync(0xffffffffu, row == -1);
-                        const bool fast = (t + 1) * S::keys <= u.free_end && !none;
+                        const bool whole = (t + 1) * S::keys <= u.free_end && !none;
                         const int b = seq % S::nbuf;
-                        if (seq >= S::nbuf) wait_empty(b, (seq / S::nbuf - 1) & 1);
-                        if (warp == 8) {
-                            uint64_t *bk = fast ? &sh.full[0][b] : &sh.partial, *bv = fast ? &sh.full[1][b] : &sh.partial;
-                            if (lane == 0) {
-                                uint64_t bad = 0;
-                                for (int i = 0; i < boxes; ++i)
-                                    if ((none >> i) & 1) bad |= (box == 64 ? ~uint64_t(0) : (uint64_t(1) << box) - 1) << (i * box);
-                                sh.bad[seq & 7][0] = uint32_t(bad);
-                                sh.bad[seq & 7][1] = uint32_t(bad >> 32);
-                                if (bad) flag_bad_page();
-                                const int bytes = __popc(live) * box * D * 2;
-                                if (fast) {
-                                    mbar_arrive_expect_tx(bk, bytes);
-                                    mbar_arrive_expect_tx(bv, bytes);
-                                } else {
-                                    mbar_arrive_expect_tx(bk, 2 * bytes);
-                                }
-                            }
-                            __syncwarp();
-                            for (int i = 0; i < boxes; ++i) {
-                                const int y = int(__shfl_sync(0xffffffffu, row, i));
-                                if (y >= 0 && elect_one()) {
-#pragma unroll
-                                    for (int j = 0; j < S::blocks; ++j) {
-                                        tma_box(place(0, b, i * box, 8 * j), &map_k, 64 * j, y, bk);
-                                        tma_box(place(1, b, i * box, 8 * j), &map_v, 64 * j, y, bv);
-                                    }
-                                }
-                                __syncwarp();
-                            }
-                        } else if (fast && lane == 0) {
-                            mbar_arrive(&sh.full[0][b]);
-                            mbar_arrive(&sh.full[1][b]);
+                        if (warp == 8 && lane == 0) {
+                            uint64_t bad = 0;
+                            for (int i = 0; none && i < boxes; ++i)
+                                if ((none >> i) & 1) bad |= (box == 64 ? ~uint64_t(0) : (uint64_t(1) << box) - 1) << (i * box);
+                            sh.bad[seq & 7][0] = uint32_t(bad);
+                            sh.bad[seq & 7][1] = uint32_t(bad >> 32);
+                            if (bad) flag_bad_page();
                         }
-                        if (!fast) {
-                            tile_wait(&sh, &sh.partial, partial++ & 1, limit_ns);
-                            loaders_sync();  // nobody arms it again before all have seen this phase
-                            clean(u, t, b);
-                            announce_both(b);
+#pragma unroll
+                        for (int job = 0; job < S::jobs; ++job) {
+                            const bool keys = job == 0, values = job == S::jobs - 1;
+                            const bool direct = whole || !values;  // (keys need no cleaning: they are masked)
+                            wait_empty(job, b);
+                            if (warp == 8) {
+                                uint64_t *bar = direct ? &sh.full[job][b] : &sh.partial;
+                                if (lane == 0) mbar_arrive_expect_tx(bar, __popc(live) * box * D * 2 * (int(keys) + int(values)));
+                                __syncwarp();
+                                for (int i = 0; i < boxes; ++i) {
+                                    const int y = int(__shfl_sync(0xffffffffu, row, i));
+                                    if (y >= 0 && elect_one()) {
+#pragma unroll
+                                        for (int j = 0; j < S::blocks; ++j) {
+                                            if (keys) tma_box(place(0, b, i * box, 8 * j), &map_k, 64 * j, y, bar);
+                                            if (values) tma_box(place(1, b, i * box, 8 * j), &map_v, 64 * j, y, bar);
+                                        }
+                                    }
+                                    __syncwarp();
+                                }
+                            } else if (direct && lane == 0) {
+                                mbar_arrive(&sh.full[job][b]);
+                            }
+                            if (!direct) {
+                                tile_wait(&sh, &sh.partial, partial++ & 1, limit_ns);
+                                loaders_sync();  // nobody arms it again before all have seen this phase
+                                clean(u, t, b);
+                                announce(job, b);
+                            }
                         }
                     }
                     attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
@@ -554,22 +580,24 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 constexpr int ALL = 2 * S::keys * CH, depth = S::nbuf > 2 ? 2 : 1;
                 int pending = 0;
                 auto settle = [&](int left) {  // announces all but the newest `left` tiles, whose copies are done
-                    for (; pending > left; --pending) announce_both((seq - pending) % S::nbuf);
+                    for (; pending > left; --pending)
+                        for (int job = 0; job < S::jobs; ++job) announce(job, (seq - pending) % S::nbuf);
                 };
                 while (p.b < bt.batch && p.unit0 < hi) {
                     const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
                     ++unit;
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    settle(0);
+                    load_q(u);
                     for (int t = u.t0; t < u.t1; ++t) {
                         const int b = seq % S::nbuf;
-                        if (seq >= S::nbuf) {
-                            const uint32_t parity = (seq / S::nbuf - 1) & 1;
-                            // (a product may wait for a pending tile before it frees this one's buffers)
-                            if (pending && !__all_sync(0xffffffffu, mbar_test(&sh.empty[1][b], parity))) {
-                                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                                settle(0);
-                            }
-                            wait_empty(b, parity);
+                        // (a product may wait for a pending tile before it frees this one's buffers)
+                        if (pending && seq >= S::nbuf &&
+                            !__all_sync(0xffffffffu, mbar_test(&sh.empty[S::jobs - 1][b], (seq / S::nbuf - 1) & 1))) {
+                            asm volatile("cp.async.wait_group 0;" ::: "memory");
+                            settle(0);
                         }
+                        for (int job = 0; job < S::jobs; ++job) wait_empty(job, b);
                         const int key = t * S::keys + tid;
                         share_bad(tid < S::keys && row_of(u, key, page_of(u, key)) == -1);
 #pragma unroll 8
@@ -586,7 +614,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             settle(0);
                             loaders_sync();  // a thread cleans what others copied, by the mask that others wrote
                             clean(u, t, b);
-                            announce_both(b);
+                            for (int job = 0; job < S::jobs; ++job) announce(job, b);
                             ++seq;
                         } else {
                             ++seq;
@@ -603,7 +631,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
         } else {
             // 16 bytes of codes a turn: 16 (Q8_0) or 32 (Q4_0) values, two or four chunks; a thread has one chunk of R
-            // keys, 128 / CH apart.  Pages of 16 keys and more come through raw buffers that warp 13 fills by bulk copies:
+            // keys, 128 / CH apart.  Pages of 16 keys and more come through raw buffers that warp 14 fills by bulk copies:
             // beside 200 KB of shared memory L1 is too small to have many plain loads on their way (they took 1.5 us a
             // tile, more than the softmax).
             constexpr int RB = S::rb, CH = RB / 16, R = S::keys * CH / LT, STEP = LT / CH;
@@ -623,7 +651,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 for (int i = 0; i < R; ++i) pages[i] = page_of(u, t * S::keys + r0 + i * STEP);
             };
             constexpr uint32_t flip = KIND == kKvQ8_0 ? 0x80808080u : 0;
-            // a job's codes from the raw buffer that warp 13 had filled
+            // a job's codes from the raw buffer that warp 14 had filled
             auto from_raw = [&](const TileUnit<KIND, D> &u, int t) {
                 const int slot = taken % S::nraw;
                 tile_wait(&sh, &sh.raw_full[slot], (taken / S::nraw) & 1, limit_ns);
@@ -671,11 +699,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             };
             auto widen = [&](int job, bool check) {
                 const int b = seq % S::nbuf;
-                if (seq >= S::nbuf) {
-                    const uint32_t parity = (seq / S::nbuf - 1) & 1;
-                    // (a tile's keys are free before its values)
-                    tile_wait(&sh, &sh.empty[jobs == 1 || job == 1][b], parity, limit_ns);
-                }
+                if (seq >= S::nbuf) tile_wait(&sh, &sh.empty[job][b], (seq / S::nbuf - 1) & 1, limit_ns);
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
@@ -705,12 +729,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         *reinterpret_cast<uint4 *>(place(kv, b, r, ch * OUT + j)) =
                             make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
                 }
-                announce(jobs == 1 ? 0 : job, b);
-                if (jobs == 1 && lane == 0) mbar_arrive(&sh.full[1][b]);
+                announce(job, b);
             };
             while (p.b < bt.batch && p.unit0 < hi) {
                 const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
                 ++unit;
+                load_q(u);
                 if (bulk) {
                     for (int t = u.t0; t < u.t1; ++t, ++seq)
                         for (int job = 0; job < jobs; ++job, ++taken) {
@@ -746,95 +770,81 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
         }
     } else {
-        if (warp == 12 && elect_one()) {
+        const int w = warp - 12;  // row tile of the products that warp 12 or 13 issues
+        if (w < S::nq && elect_one()) {
             // ================= products ================================================================
             constexpr uint32_t fmt = BF ? 1 : 0;
             constexpr uint32_t idesc0 = (1u << 4) | (fmt << 7) | (fmt << 10) | (8u << 24);
             constexpr uint32_t id_qk = idesc0 | (uint32_t(S::keys / 8) << 17);
             constexpr uint32_t id_pv = idesc0 | (1u << 16) | (uint32_t(D / 8) << 17);  // V: its columns are contiguous
-            uint32_t nb = 0, nq[2] = {0, 0}, np[2][2] = {};  // tiles, units, tiles by turn
-            const uint32_t q0 = smem_desc_lo(smem_u32(sq), 16), k0 = smem_desc_lo(smem_u32(sbuf), 16),
+            uint32_t nb = 0, units = 0, np[2] = {0, 0};  // tiles, units, tiles by turn
+            const uint32_t q0 = smem_desc_lo(smem_u32(sq + w * 128 * 128), 16), k0 = smem_desc_lo(smem_u32(sbuf), 16),
                            v0 = smem_desc_lo(smem_u32(sbuf + S::nbuf * S::buf), S::keys * 128);
-            auto qk = [&](int w, int x, uint32_t b) {
-                const uint32_t a = q0 + ((w * 128 * 128) >> 4), k = k0 + b * (S::buf >> 4);
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    mma_ss(tmem + (w * 2 + x) * S::s_cols, smem_desc(a + (((i >> 2) * (S::rows * 128) + (i & 3) * 32) >> 4)),
-                           smem_desc(k + (((i >> 2) * (S::keys * 128) + (i & 3) * 32) >> 4)), id_qk, i > 0);
-                mma_commit(&sh.s_full[w][x]);
-            };
-            auto pv = [&](int w, int x, uint32_t b, bool acc) {
-                const uint32_t v = v0 + b * (S::buf >> 4);
-#pragma unroll
-                for (int i = 0; i < S::keys / 16; ++i)
-                    mma_ts(tmem + S::o_col + w * S::o_cols, tmem + (w * 2 + x) * S::s_cols + i * 8,
-                           smem_desc(v + ((i * 2048) >> 4)), id_pv, acc || i > 0);
-                mma_commit(&sh.pv_done[w][x]);
-            };
-            auto wait_full = [&](int kv, uint32_t n) {
-                tile_wait(&sh, &sh.full[kv][n % S::nbuf], (n / S::nbuf) & 1, limit_ns);
-                fence_after();
-            };
+            const uint32_t ts = tmem + w * 2 * S::s_cols, to = tmem + S::o_col + w * S::o_cols;
             while (p.b < bt.batch && p.unit0 < hi) {
                 const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
-                const int tiles = u.t1 - u.t0, active = S::nq == 2 && u.nrows > 128 ? 2 : 1;
-#pragma unroll
-                for (int w = 0; w < S::nq; ++w)
-                    if (w < active) tile_wait(&sh, &sh.q_full[w], nq[w]++ & 1, limit_ns);
-                auto scores = [&](int i, int w) { qk(w, i & 1, (nb + i) % S::nbuf); };
-                auto values = [&](int i, int w) {
-                    if (i & 1) tile_wait(&sh, &sh.p_full[w][1], np[w][1]++ & 1, limit_ns);
-                    else tile_wait(&sh, &sh.p_full[w][0], np[w][0]++ & 1, limit_ns);
+                const int tiles = u.t1 - u.t0;
+                const bool on = w * 128 < u.nrows;  // (else this warp only keeps step)
+                auto wait_full = [&](int job, int i) {
+                    tile_wait(&sh, &sh.full[job][(nb + i) % S::nbuf], ((nb + i) / S::nbuf) & 1, limit_ns);
                     fence_after();
-                    pv(w, i & 1, (nb + i) % S::nbuf, i > 0);
                 };
-                if constexpr (S::nq == 2) {
-                    // Two tiles ahead of the softmax: when a row tile's P V of tile i is issued, its columns take the scores
-                    // of tile i + 2, while the softmax works on those of i + 1.  Row tiles do not wait for each other.
-                    for (int i = 0; i < min(tiles, 2); ++i) {
-                        wait_full(0, nb + i);
+                auto done = [&](uint64_t *bar) {
+                    if (on) mma_commit(bar);
+                    else mbar_arrive(bar);
+                };
+                auto scores = [&](int i) {  // S of tile i, once its keys are there
+                    wait_full(0, i);
+                    const uint32_t k = k0 + (nb + i) % S::nbuf * (S::buf >> 4), d = ts + (i & 1) * S::s_cols;
+                    if (on) {
 #pragma unroll
-                        for (int w = 0; w < 2; ++w)
-                            if (w < active) scores(i, w);
-                        mma_commit(&sh.empty[0][(nb + i) % S::nbuf]);
+                        for (int j = 0; j < D / 16; ++j)
+                            mma_ss(d, smem_desc(q0 + (((j >> 2) * (S::rows * 128) + (j & 3) * 32) >> 4)),
+                                   smem_desc(k + (((j >> 2) * (S::keys * 128) + (j & 3) * 32) >> 4)), id_qk, j > 0);
+                        mma_commit(&sh.s_full[w][i & 1]);
                     }
-                    for (int i = 0; i < tiles; ++i) {
-                        const bool more = i + 2 < tiles;
+                    if (S::jobs == 2) done(&sh.empty[0][(nb + i) % S::nbuf]);
+                    if (i + 1 == tiles) done(&sh.q_free);
+                };
+                auto outputs = [&](int i) {  // O += P V of tile i, once its weights are there
+                    if (S::jobs == 2) wait_full(1, i);
+                    if (on) {
+                        if (i & 1) tile_wait(&sh, &sh.p_full[w][1], np[1]++ & 1, limit_ns);
+                        else tile_wait(&sh, &sh.p_full[w][0], np[0]++ & 1, limit_ns);
+                        fence_after();
+                        const uint32_t v = v0 + (nb + i) % S::nbuf * (S::buf >> 4), a = ts + (i & 1) * S::s_cols;
 #pragma unroll
-                        for (int w = 0; w < 2; ++w)
-                            if (w < active) {
-                                if (w == 0) wait_full(1, nb + i);
-                                values(i, w);
-                                if (more) {
-                                    if (w == 0) wait_full(0, nb + i + 2);
-                                    scores(i + 2, w);
-                                }
-                            }
-                        mma_commit(&sh.empty[1][(nb + i) % S::nbuf]);
-                        if (more) mma_commit(&sh.empty[0][(nb + i + 2) % S::nbuf]);
+                        for (int j = 0; j < S::keys / 16; ++j)
+                            mma_ts(to, a + j * 8, smem_desc(v + ((j * 2048) >> 4)), id_pv, i > 0 || j > 0);
+                        mma_commit(&sh.pv_done[w][i & 1]);
+                    }
+                    done(&sh.empty[S::jobs - 1][(nb + i) % S::nbuf]);
+                };
+                tile_wait(&sh, &sh.q_full, units++ & 1, limit_ns);
+                if constexpr (S::jobs == 1) {
+                    // Two tiles ahead of the softmax: when P V of tile i is issued, its columns take the scores of tile
+                    // i + 2, while the softmax works on those of i + 1.
+                    for (int i = 0; i < min(tiles, 2); ++i) scores(i);
+                    for (int i = 0; i < tiles; ++i) {
+                        outputs(i);
+                        if (i + 2 < tiles) scores(i + 2);
                     }
                 } else {
-                    // One tile ahead (two buffers of each kind): S of tile i + 1 goes to the other turn's columns, whose P
-                    // was read by the products of tile i - 1, which were issued before.
-                    for (int i = -1; i < tiles; ++i) {
-                        if (i + 1 < tiles) {
-                            wait_full(0, nb + i + 1);
-                            scores(i + 1, 0);
-                            mma_commit(&sh.empty[0][(nb + i + 1) % S::nbuf]);
-                        }
-                        if (i < 0) continue;
-                        wait_full(1, nb + i);
-                        values(i, 0);
-                        mma_commit(&sh.empty[1][(nb + i) % S::nbuf]);
+                    // One tile ahead (two buffers): S of tile i + 1 goes to the other turn's columns, whose P was read by the
+                    // products of tile i - 1, which were issued before.
+                    scores(0);
+                    for (int i = 0; i < tiles; ++i) {
+                        if (i + 1 < tiles) scores(i + 1);
+                        outputs(i);
                     }
                 }
                 nb += tiles;
                 attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
             }
-            mma_commit(&sh.drain);
-            tile_wait(&sh, &sh.drain, 0, limit_ns);
+            mma_commit(&sh.drain[w]);
+            tile_wait(&sh, &sh.drain[w], 0, limit_ns);
         }
-        if (warp == 13 && S::quant && c.page_shift >= kTileBulkShift) {
+        if (warp == 14 && S::quant && c.page_shift >= kTileBulkShift) {
             // ================= raw buffers: bulk copies, page by page ====================================
             const int per = min(S::keys, 1 << c.page_shift), parts = S::keys / per;  // keys of a copy, copies of a tile
             uint32_t filled = 0;
