@@ -223,19 +223,18 @@ __device__ __forceinline__ int64_t attn_locate(const KvCacheView &c, const KvBat
     return work;
 }
 
-// The unit behind p's; b reaches bt.batch behind the last.  (The sequence is looked up again rather than kept in
-// registers through a unit.)
+// The unit behind p's; b reaches bt.batch behind the last.  seq: p's sequence, looked up again only where it changes.
 template <int ROWS, int KEYS, int COST>
-__device__ __forceinline__ void attn_next(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, AttnPos &p) {
-    const AttnSeq<ROWS, KEYS> q(load_seq(bt, c, p.b), io);
+__device__ __forceinline__ void attn_next(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, AttnPos &p, KvSeq &seq) {
+    const AttnSeq<ROWS, KEYS> q(seq, io);
     p.unit0 += q.key_tiles(p.mt) + COST;
     if (++p.mt < q.tiles) return;
     p.mt = 0;
     if (++p.head < c.kv_heads) return;
     p.head = 0;
     for (++p.b; p.b < bt.batch; ++p.b) {
-        const KvSeq s = load_seq(bt, c, p.b);
-        if (s.q1 > s.q0) return;
+        seq = load_seq(bt, c, p.b);
+        if (seq.q1 > seq.q0) return;
     }
 }
 

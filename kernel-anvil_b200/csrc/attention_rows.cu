@@ -143,10 +143,11 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
     if (int(blockIdx.x) >= shares.ctas) return;
     const int64_t lo = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
     AttnPos p = sc.pos;
+    KvSeq kseq = load_seq(bt, c, p.b);
     int slot = 0, fill = 0;     // ring slots: next to be worked on, next to be filled
 
     while (p.b < bt.batch && p.unit0 < hi) {
-        const AttnSeq<ROWS, kRowsKeys> q(load_seq(bt, c, p.b), io);
+        const AttnSeq<ROWS, kRowsKeys> q(kseq, io);
         const int ntiles = q.key_tiles(p.mt), nkeys = q.keys(p.mt);
         const int t0 = int(max(lo - p.unit0, int64_t(0))), t1 = int(min(hi - p.unit0, int64_t(ntiles)));
         const int key_end = min(t1 * kRowsKeys, nkeys);
@@ -618,7 +619,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
             }
         }
         __syncthreads();  // before the rings are filled again
-        attn_next<ROWS, kRowsKeys, kRowsCost>(c, bt, io, p);
+        attn_next<ROWS, kRowsKeys, kRowsCost>(c, bt, io, p, kseq);
     }
 }
 

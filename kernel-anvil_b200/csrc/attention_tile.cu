@@ -124,7 +124,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
 
 struct TileShared {
     AttnScratch sc;
-    uint64_t full[2][4], empty[2][4], raw_full[3], raw_empty[3], partial, q_full, q_free,  // [job][buffer]
+    uint64_t full[2][4], empty[2][4], raw_full[3], raw_empty[3], partial[4], q_full, q_free,  // [job][buffer]
          s_full[2][2], p_full[2][2], pv_done[2][2], drain[2];  // [row tile][turn]
     float fac[2][256];      // [unit % 2]: what a row's scores are multiplied by
     uint32_t tmem;
@@ -183,9 +183,8 @@ template <int KIND, int D> struct TileUnit {
     using S = TileShape<KIND, D>;
     AttnSeq<S::rows, S::keys> q;
     int ntiles, t0, t1, key_end, nrows, free_end;
-    __device__ __forceinline__ TileUnit(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, const AttnPos &p,
-                                        int64_t lo, int64_t hi)
-        : q(load_seq(bt, c, p.b), io) {
+    __device__ __forceinline__ TileUnit(const KvSeq &seq, const AttnIO &io, const AttnPos &p, int64_t lo, int64_t hi)
+        : q(seq, io) {
         ntiles = q.key_tiles(p.mt);
         t0 = int(max(lo - p.unit0, int64_t(0)));
         t1 = int(min(hi - p.unit0, int64_t(ntiles)));
@@ -215,6 +214,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     if (int(blockIdx.x) >= shares.ctas) return;
     const int64_t lo = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
     AttnPos p = sh.sc.pos;
+    KvSeq kseq = load_seq(bt, c, p.b);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::nbuf; ++i)
@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 mbar_init(&sh.pv_done[i][x], 1);
             }
         }
-        mbar_init(&sh.partial, 1);
-        mbar_init(&sh.q_full, kTileLoaders / 32);
+        for (int i = 0; i < 4; ++i) mbar_init(&sh.partial[i], 1);
+        mbar_init(&sh.q_full, (S::quant ? kTileLoaders : kTileLoaders - 32) / 32);
         mbar_init(&sh.q_free, S::nq);
         for (int i = 0; i < 2; ++i) mbar_init(&sh.drain[i], 1);
         mbar_fence_init();
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         int unit = 0, seq = 0;              // units and key tiles so far, counted alike in every role
         if (w < S::nq)
             while (p.b < bt.batch && p.unit0 < hi) {
-                const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                const TileUnit<KIND, D> u(kseq, io, p, lo, hi);
                 ++unit;
                 if (w * 128 < u.nrows) {
                     const int ur = w * 128 + r;
@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     fence_before();
                 }
                 seq += u.t1 - u.t0;
-                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p, kseq);
             }
     } else if (warp < 12) {
         // ================= loaders: keys and values of a tile together ===============================
@@ -440,48 +440,65 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             }
         };
         // A unit's query rows into the swizzled operand, while the softmax is still at the unit before: once that one's
-        // scores are all taken.  Rows that are none are zeros.
+        // scores are all taken.  Rows that are none are zeros.  (16-bit caches: by warps 9-11.)
         auto load_q = [&](const TileUnit<KIND, D> &u) {
-            constexpr int CHQ = D / 8, FLY = 4;
+            constexpr int CHQ = D / 8, QT = S::quant ? LT : LT - 32, FLY = 8;
+            const int qt = tid - (LT - QT);
             if (unit > 1) {
                 tile_wait(&sh, &sh.q_free, unit & 1, limit_ns);
                 __syncwarp();
             }
             const int all = (u.nrows > 128 ? S::rows : 128) * CHQ;
-            for (int at0 = tid; at0 < all; at0 += FLY * LT) {
-                uint4 x[FLY];
-#pragma unroll
-                for (int f = 0; f < FLY; ++f) {
-                    const int at = at0 + f * LT, ur = at / CHQ, ch = at % CHQ;
-                    const unsigned rr = unsigned(p.mt) * S::rows + ur;
-                    const int tok = int(rr / unsigned(u.q.group)), h = p.head * u.q.group + int(rr - unsigned(tok) * u.q.group);
-                    x[f] = ur < u.nrows ? __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(io.q) +
-                                                (u.q.s.q0 + int64_t(tok)) * io.q_row + h * io.q_head) + ch)
-                                        : make_uint4(0, 0, 0, 0);
+            auto row_at = [&](int ur) {
+                const unsigned rr = unsigned(p.mt) * S::rows + ur;
+                const int tok = int(rr / unsigned(u.q.group)), h = p.head * u.q.group + int(rr - unsigned(tok) * u.q.group);
+                return static_cast<const uint16_t *>(io.q) + (u.q.s.q0 + int64_t(tok)) * io.q_row + h * io.q_head;
+            };
+            auto place_q = [&](int ur, int ch) { return sq + (ch >> 3) * (S::rows * 128) + ur * 128 + (((ch & 7) ^ (ur & 7)) << 4); };
+            // (above zero, so that a masked score stays -inf)
+            auto put_fac = [&](int ur, int ex) { sh.fac[unit & 1][ur] = fmaxf(fabsf(io.scale_log2) * pow2i(-ex), 1e-36f); };
+            // a negative scale: -q, so that the largest score stays the largest
+            const uint32_t sign = io.scale_log2 < 0.0f ? 0x80008000u : 0;
+            if (sign == 0 && !(S::quant && io.q_bf16)) {
+#pragma unroll 8
+                for (int at = qt; at < all; at += QT) {
+                    const int ur = at / CHQ, ch = at % CHQ;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(place_q(ur, ch))),
+                                 "l"(ur < u.nrows ? row_at(ur) + ch * 8 : io.q), "r"(ur < u.nrows ? 16 : 0)
+                                 : "memory");
+                    if (ch == 0) put_fac(ur, 0);
                 }
+                asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+            } else {
+                for (int at0 = qt; at0 < all + qt; at0 += FLY * QT) {  // (every lane the same number of times)
+                    uint4 x[FLY];
 #pragma unroll
-                for (int f = 0; f < FLY; ++f) {
-                    const int at = at0 + f * LT, ur = at / CHQ, ch = at % CHQ;
-                    uint32_t y[4] = {x[f].x, x[f].y, x[f].z, x[f].w};
-                    int ex = 0;
-                    if (S::quant && io.q_bf16) {
-                        uint32_t m = 0;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) m = max(max(m, y[j] & 0x7FFFu), (y[j] >> 16) & 0x7FFFu);
-#pragma unroll
-                        for (int o = CHQ / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        ex = q_exponent(m << 16);
-                        const float up = pow2i(ex);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            y[j] = pack_half(__uint_as_float(y[j] << 16) * up, __uint_as_float(y[j] & 0xFFFF0000u) * up);
+                    for (int f = 0; f < FLY; ++f) {
+                        const int at = at0 + f * QT, ur = at / CHQ, ch = at % CHQ;
+                        x[f] = at < all && ur < u.nrows ? __ldg(reinterpret_cast<const uint4 *>(row_at(ur)) + ch) : make_uint4(0, 0, 0, 0);
                     }
-                    // a negative scale: -q, so that the largest score stays the largest
-                    const uint32_t sign = io.scale_log2 < 0.0f ? 0x80008000u : 0;
-                    *reinterpret_cast<uint4 *>(sq + (ch >> 3) * (S::rows * 128) + ur * 128 + (((ch & 7) ^ (ur & 7)) << 4)) =
-                        make_uint4(y[0] ^ sign, y[1] ^ sign, y[2] ^ sign, y[3] ^ sign);
-                    // (above zero, so that a masked score stays -inf)
-                    if (ch == 0) sh.fac[unit & 1][ur] = fmaxf(fabsf(io.scale_log2) * pow2i(-ex), 1e-36f);
+#pragma unroll
+                    for (int f = 0; f < FLY; ++f) {
+                        const int at = at0 + f * QT, ur = at / CHQ, ch = at % CHQ;
+                        uint32_t y[4] = {x[f].x, x[f].y, x[f].z, x[f].w};
+                        int ex = 0;
+                        if (S::quant && io.q_bf16) {
+                            uint32_t m = 0;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) m = max(max(m, y[j] & 0x7FFFu), (y[j] >> 16) & 0x7FFFu);
+#pragma unroll
+                            for (int o = CHQ / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+                            ex = q_exponent(m << 16);
+                            const float up = pow2i(ex);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                y[j] = pack_half(__uint_as_float(y[j] << 16) * up, __uint_as_float(y[j] & 0xFFFF0000u) * up);
+                        }
+                        if (at < all) {
+                            *reinterpret_cast<uint4 *>(place_q(ur, ch)) = make_uint4(y[0] ^ sign, y[1] ^ sign, y[2] ^ sign, y[3] ^ sign);
+                            if (ch == 0) put_fac(ur, ex);
+                        }
+                    }
                 }
             }
             fence_async();
@@ -498,11 +515,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             // Of a tile that some row does not see whole, or that lacks pages, what is not finite and what is no key
             // leaves the values first (see the outputs).
             constexpr int CH = D / 8;
-            auto clean = [&](const TileUnit<KIND, D> &u, int t, int b) {
+            auto clean = [&](const TileUnit<KIND, D> &u, int t, int b, int from) {  // by threads `from` and up
                 const int left = u.key_end - t * S::keys;
                 const uint32_t bad[2] = {sh.bad[seq & 7][0], sh.bad[seq & 7][1]};
 #pragma unroll 2
-                for (int at = tid; at < S::keys * CH; at += LT) {
+                for (int at = tid - from; at < S::keys * CH; at += LT - from) {
                     const int r = at / CH;
                     uint4 *w4 = reinterpret_cast<uint4 *>(place(1, b, r, at % CH));
                     const uint4 x = *w4;
@@ -521,12 +538,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 __syncwarp();
             };
             if (box) {
+                // Warp 8 issues the copies; the other three load the queries and clean, and do not hold it up.
                 const int boxes = S::keys / box;  // of a tile's keys
-                uint32_t partial = 0;             // tiles that were cleaned
+                uint32_t partial = 0;             // bit b: parity of the next partial tile in buffer b
                 while (p.b < bt.batch && p.unit0 < hi) {
-                    const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                    const TileUnit<KIND, D> u(kseq, io, p, lo, hi);
                     ++unit;
-                    load_q(u);
+                    if (warp > 8) load_q(u);
                     // lane i: the page of box i
                     int page = lane < boxes ? page_of(u, u.t0 * S::keys + lane * box) : 0;
                     for (int t = u.t0; t < u.t1; ++t, ++seq) {
@@ -535,22 +553,25 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         const uint32_t live = __ballot_sync(0xffffffffu, row >= 0), none = __ballot_sync(0xffffffffu, row == -1);
                         const bool whole = (t + 1) * S::keys <= u.free_end && !none;
                         const int b = seq % S::nbuf;
-                        if (warp == 8 && lane == 0) {
-                            uint64_t bad = 0;
-                            for (int i = 0; none && i < boxes; ++i)
-                                if ((none >> i) & 1) bad |= (box == 64 ? ~uint64_t(0) : (uint64_t(1) << box) - 1) << (i * box);
-                            sh.bad[seq & 7][0] = uint32_t(bad);
-                            sh.bad[seq & 7][1] = uint32_t(bad >> 32);
-                            if (bad) flag_bad_page();
-                        }
 #pragma unroll
                         for (int job = 0; job < S::jobs; ++job) {
                             const bool keys = job == 0, values = job == S::jobs - 1;
                             const bool direct = whole || !values;  // (keys need no cleaning: they are masked)
                             wait_empty(job, b);
                             if (warp == 8) {
-                                uint64_t *bar = direct ? &sh.full[job][b] : &sh.partial;
-                                if (lane == 0) mbar_arrive_expect_tx(bar, __popc(live) * box * D * 2 * (int(keys) + int(values)));
+                                uint64_t *bar = direct ? &sh.full[job][b] : &sh.partial[b];
+                                if (lane == 0) {
+                                    if (job == 0) {
+                                        uint64_t bad = 0;
+                                        for (int i = 0; none && i < boxes; ++i)
+                                            if ((none >> i) & 1) bad |= (box == 64 ? ~uint64_t(0) : (uint64_t(1) << box) - 1) << (i * box);
+                                        sh.bad[seq & 7][0] = uint32_t(bad);
+                                        sh.bad[seq & 7][1] = uint32_t(bad >> 32);
+                                        if (bad) flag_bad_page();
+                                    }
+                                    mbar_arrive_expect_tx(bar, __popc(live) * box * D * 2 * (int(keys) + int(values)));
+                                    if (!direct) mbar_arrive(&sh.full[job][b]);
+                                }
                                 __syncwarp();
                                 for (int i = 0; i < boxes; ++i) {
                                     const int y = int(__shfl_sync(0xffffffffu, row, i));
@@ -563,18 +584,18 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                     }
                                     __syncwarp();
                                 }
-                            } else if (direct && lane == 0) {
-                                mbar_arrive(&sh.full[job][b]);
-                            }
-                            if (!direct) {
-                                tile_wait(&sh, &sh.partial, partial++ & 1, limit_ns);
-                                loaders_sync();  // nobody arms it again before all have seen this phase
-                                clean(u, t, b);
+                            } else if (direct) {
+                                if (lane == 0) mbar_arrive(&sh.full[job][b]);
+                            } else {
+                                tile_wait(&sh, &sh.partial[b], (partial >> b) & 1, limit_ns);
+                                __syncwarp();
+                                partial ^= 1u << b;
+                                clean(u, t, b, 32);
                                 announce(job, b);
                             }
                         }
                     }
-                    attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
+                    attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p, kseq);
                 }
             } else {
                 constexpr int ALL = 2 * S::keys * CH, depth = S::nbuf > 2 ? 2 : 1;
@@ -584,11 +605,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         for (int job = 0; job < S::jobs; ++job) announce(job, (seq - pending) % S::nbuf);
                 };
                 while (p.b < bt.batch && p.unit0 < hi) {
-                    const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                    const TileUnit<KIND, D> u(kseq, io, p, lo, hi);
                     ++unit;
                     asm volatile("cp.async.wait_group 0;" ::: "memory");
                     settle(0);
-                    load_q(u);
+                    if (warp > 8) load_q(u);
                     for (int t = u.t0; t < u.t1; ++t) {
                         const int b = seq % S::nbuf;
                         // (a product may wait for a pending tile before it frees this one's buffers)
@@ -613,7 +634,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             asm volatile("cp.async.wait_group 0;" ::: "memory");
                             settle(0);
                             loaders_sync();  // a thread cleans what others copied, by the mask that others wrote
-                            clean(u, t, b);
+                            clean(u, t, b, 0);
                             for (int job = 0; job < S::jobs; ++job) announce(job, b);
                             ++seq;
                         } else {
@@ -624,7 +645,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             }
                         }
                     }
-                    attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
+                    attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p, kseq);
                 }
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
                 settle(0);
@@ -732,7 +753,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 announce(job, b);
             };
             while (p.b < bt.batch && p.unit0 < hi) {
-                const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                const TileUnit<KIND, D> u(kseq, io, p, lo, hi);
                 ++unit;
                 load_q(u);
                 if (bulk) {
@@ -766,7 +787,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         widen(jobs - 1, check);
                     }
                 }
-                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p, kseq);
             }
         }
     } else {
@@ -782,7 +803,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                            v0 = smem_desc_lo(smem_u32(sbuf + S::nbuf * S::buf), S::keys * 128);
             const uint32_t ts = tmem + w * 2 * S::s_cols, to = tmem + S::o_col + w * S::o_cols;
             while (p.b < bt.batch && p.unit0 < hi) {
-                const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                const TileUnit<KIND, D> u(kseq, io, p, lo, hi);
                 const int tiles = u.t1 - u.t0;
                 const bool on = w * 128 < u.nrows;  // (else this warp only keeps step)
                 auto wait_full = [&](int job, int i) {
@@ -839,7 +860,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 }
                 nb += tiles;
-                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p, kseq);
             }
             mma_commit(&sh.drain[w]);
             tile_wait(&sh, &sh.drain[w], 0, limit_ns);
@@ -850,7 +871,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             uint32_t filled = 0;
             int seq = 0;
             while (p.b < bt.batch && p.unit0 < hi) {
-                const TileUnit<KIND, D> u(c, bt, io, p, lo, hi);
+                const TileUnit<KIND, D> u(kseq, io, p, lo, hi);
                 auto page_of = [&](int t) {  // lane i: the page of part i
                     const int key = t * S::keys + lane * per;
                     return lane < parts && key < u.key_end ? __ldg(bt.table + p.b * bt.table_stride + (key >> c.page_shift)) : -1;
@@ -896,7 +917,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         }
                     }
                 }
-                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p);
+                attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p, kseq);
             }
             // (every copy has landed before the loaders, and so the CTA, are done)
         }
