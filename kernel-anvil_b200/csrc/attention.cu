@@ -89,14 +89,16 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
     if (!q || !out || !bv.kv_len) return fail(ANVIL_ERR_INVALID, "null q, out or kv_len");
     if (!std::isfinite(scale)) return fail(ANVIL_ERR_INVALID, "scale=%f is not finite", double(scale));
     const auto mis = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
-    if (mis(q) || mis(out) || mis(workspace) || q_row_stride % 8 || q_head_stride % 8)
-        return fail(ANVIL_ERR_ALIGN, "q, its rows, out and the workspace must be 16-byte aligned");
+    if (mis(q) || mis(out) || q_row_stride % 8 || q_head_stride % 8)
+        return fail(ANVIL_ERR_ALIGN, "q, its rows and out must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(workspace) % 32) return fail(ANVIL_ERR_ALIGN, "the workspace must be 32-byte aligned");
     const AttnPlan p = attn_plan(cache, cv, bv, heads);
     if (p.bytes && (!workspace || workspace_bytes < p.bytes))
         return fail(ANVIL_ERR_INVALID, "a workspace of %lld bytes is needed, got %lld", (long long)p.bytes,
                     (long long)(workspace ? workspace_bytes : 0));
-    const AttnIO io{q, q_row_stride, q_head_stride, out, heads, heads / cv.kv_heads, scale * 1.4426950408889634f,
-                    causal != 0, dtype == kKvBF16, static_cast<float *>(workspace)};
+    AttnIO io{q, q_row_stride, q_head_stride, out, heads, 0, 0, 0, scale * 1.4426950408889634f,
+              causal != 0, dtype == kKvBF16, static_cast<float *>(workspace)};
+    set_group(io, heads / cv.kv_heads);
     if (!p.nt)
         return attn_tile_launch(cache->kind, cache->head_dim, cv, bv, io, p.ctas, p.join,
                                 reinterpret_cast<cudaStream_t>(stream));

@@ -27,11 +27,27 @@ struct AttnIO {
     int64_t q_row, q_head;  // in values
     void *out;              // (total, heads, D)
     int heads, group;       // group: query heads per key/value head
+    uint32_t group_mul;     // n / group = n * group_mul / 2^(32 + group_shift) for n < 2^31 (group 1: group_mul 0)
+    int group_shift;
     float scale_log2;       // scale * log2(e): scores are kept in powers of two
     int causal;
     int q_bf16;             // q and out are bf16 (else fp16)
     float *part;            // partial results, see AttnPart
 };
+
+// n / group without a division (group is the call's, and dozens of instructions as a divisor): with l the least
+// power 2^l >= group and M = floor(2^(31+l) / group) + 1, M group exceeds 2^(31+l) by at most 2^l, so n M / 2^(31+l)
+// exceeds n / group by less than 1 / group.
+__device__ __forceinline__ unsigned by_group(const AttnIO &io, unsigned n) {
+    return io.group_mul ? __umulhi(n, io.group_mul) >> io.group_shift : n;
+}
+inline void set_group(AttnIO &io, int group) {
+    io.group = group;
+    int l = 0;
+    while ((int64_t(1) << l) < group) ++l;
+    io.group_mul = group == 1 ? 0 : uint32_t((uint64_t(1) << (31 + l)) / group + 1);
+    io.group_shift = l - 1;
+}
 
 // Partial results of CTA c: slot 2 c (the unit it found begun) and 2 c + 1 (the unit it left
 // unfinished), each ROWS x (D + 2) floats: the rows' outputs, then maxima, then sums.
@@ -46,17 +62,17 @@ template <int ROWS, int D> struct AttnPart {
 // batches of 2^31 query rows).
 template <int ROWS, int KEYS> struct AttnSeq {
     KvSeq s;
-    int n, group, causal, tiles;  // new tokens; row tiles
+    int n, tiles;  // new tokens; row tiles
+    const AttnIO &io;
 
     __device__ __forceinline__ AttnSeq(const KvSeq &seq, const AttnIO &io)
-        : s(seq), n(seq.q1 - seq.q0), group(io.group), causal(io.causal),
-          tiles(int((unsigned(n) * unsigned(io.group) + ROWS - 1) / ROWS)) {}
+        : s(seq), n(seq.q1 - seq.q0), tiles(int((unsigned(n) * unsigned(io.group) + ROWS - 1) / ROWS)), io(io) {}
 
     // Keys that some row of tile mt sees (its last token's), and their key tiles: at least one,
     // so that rows without keys are visited and get their zeros.
     __device__ __forceinline__ int keys(int mt) const {
-        if (!causal) return s.kv;
-        const int last = min(n - 1, int((unsigned(mt + 1) * ROWS - 1) / unsigned(group)));
+        if (!io.causal) return s.kv;
+        const int last = min(n - 1, int(by_group(io, unsigned(mt + 1) * ROWS - 1)));
         return kv_seen(last, n, s.kv, true);
     }
     __device__ __forceinline__ int key_tiles(int mt) const { return max(1, (keys(mt) + KEYS - 1) / KEYS); }
@@ -103,10 +119,10 @@ struct AttnScratch {
 template <int ROWS, int KEYS, int COST>
 __device__ __forceinline__ int64_t attn_head_work(const AttnSeq<ROWS, KEYS> &q, bool live) {
     int64_t w = 0;
-    const bool many = live && q.causal && q.tiles > 2;
+    const bool many = live && q.io.causal && q.tiles > 2;
     if (live && !many) {
         w = q.tiles ? int64_t(q.tiles) * (q.key_tiles(0) + COST) : 0;
-        if (q.causal && q.tiles == 2) w += q.key_tiles(1) - q.key_tiles(0);
+        if (q.io.causal && q.tiles == 2) w += q.key_tiles(1) - q.key_tiles(0);
     }
     for (uint32_t rest = __ballot_sync(0xffffffffu, many); rest; rest &= rest - 1) {
         const int src = __ffs(rest) - 1, lane = threadIdx.x & 31;
@@ -194,7 +210,7 @@ __device__ __forceinline__ int64_t attn_locate(const KvCacheView &c, const KvBat
         int64_t unit = sc->at + head * per;  // place of the unit of row tile m0
         const int64_t rest = want - unit;
         AttnPos p{b, int(head), 0, 0};
-        if (!q.causal || q.tiles == 1) {
+        if (!io.causal || q.tiles == 1) {
             const int one = q.key_tiles(0) + COST;
             p.mt = int(rest / one);
             p.unit0 = unit + int64_t(p.mt) * one + COST;
@@ -358,7 +374,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(KvCacheView 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int share = np > 32 ? 8 : np > 16 ? 4 : np > 8 ? 2 : 1;  // warps of a row
     const int sub = warp % share, rows = kJoinWarps / share;        // rows at once
-    const int nrows = int(min(unsigned(ROWS), unsigned(q.n) * unsigned(q.group) - unsigned(p.mt) * ROWS));
+    const int nrows = int(min(unsigned(ROWS), unsigned(q.n) * unsigned(io.group) - unsigned(p.mt) * ROWS));
     using P = AttnPart<ROWS, D>;
     constexpr int V = D / 32;
     for (int r0 = blockIdx.y * rows; r0 < nrows; r0 += rows * gridDim.y) {
@@ -416,7 +432,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(KvCacheView 
         if (!live || sub) continue;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const unsigned r = unsigned(p.mt) * ROWS + row;
-        const int token = q.s.q0 + int(r / unsigned(q.group)), h = p.head * q.group + int(r % unsigned(q.group));
+        const int tok = int(by_group(io, r)), token = q.s.q0 + tok, h = p.head * io.group + int(r - unsigned(tok) * io.group);
         uint32_t *out = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(io.out) +
                                                      (int64_t(token) * io.heads + h) * D) + lane * (V / 2);
 #pragma unroll

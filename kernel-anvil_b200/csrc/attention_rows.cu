@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
         const int ntiles = q.key_tiles(p.mt), nkeys = q.keys(p.mt);
         const int t0 = int(max(lo - p.unit0, int64_t(0))), t1 = int(min(hi - p.unit0, int64_t(ntiles)));
         const int key_end = min(t1 * kRowsKeys, nkeys);
-        const int nrows = int(min(int64_t(ROWS), int64_t(unsigned(q.n) * unsigned(q.group) - unsigned(p.mt) * ROWS)));
+        const int nrows = int(min(int64_t(ROWS), int64_t(unsigned(q.n) * unsigned(io.group) - unsigned(p.mt) * ROWS)));
 
         // ---- the ring: step s covers keys 16 s .. 16 s + 15
         const int step0 = t0 * 4 + warp, steps = (key_end + kRowsStep - 1) / kRowsStep;
@@ -231,9 +231,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
         for (int t = 0; t < NT; ++t) {
             const int r = 8 * t + g;
             const unsigned rr = unsigned(p.mt) * ROWS + r;
-            const int tok = int(rr / unsigned(q.group)), h = p.head * q.group + int(rr - unsigned(tok) * q.group);
+            const int tok = int(by_group(io, rr)), h = p.head * io.group + int(rr - unsigned(tok) * io.group);
             const bool live = r < nrows;
-            const int my_seen = live ? kv_seen(tok, q.n, q.s.kv, q.causal) : 0;
+            const int my_seen = live ? kv_seen(tok, q.n, q.s.kv, io.causal) : 0;
             const uint16_t *src = static_cast<const uint16_t *>(io.q) + (q.s.q0 + int64_t(tok)) * io.q_row + h * io.q_head;
             uint32_t m = 0;
 #pragma unroll
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
             }
         }
         // every row of the unit sees the keys below this: no mask is needed there
-        const int free_end = min(key_end, kv_seen(int(unsigned(p.mt) * ROWS / unsigned(q.group)), q.n, q.s.kv, q.causal));
+        const int free_end = min(key_end, kv_seen(int(by_group(io, unsigned(p.mt) * ROWS)), q.n, q.s.kv, io.causal));
 
         float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -595,7 +595,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
             }
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             const unsigned rr = unsigned(p.mt) * ROWS + r;
-            const int tok = int(rr / unsigned(q.group)), h = p.head * q.group + int(rr - unsigned(tok) * q.group);
+            const int tok = int(by_group(io, rr)), h = p.head * io.group + int(rr - unsigned(tok) * io.group);
             uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(io.out) +
                                                          ((int64_t(q.s.q0) + tok) * io.heads + h) * D);
 #pragma unroll

@@ -169,6 +169,19 @@ __device__ __forceinline__ uint32_t ld_stream16(const uint8_t *p) {
     asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(v) : "l"(p));
     return v;
 }
+// 0 * a + c of 16-bit pairs
+template <bool BF> __device__ __forceinline__ uint32_t zero_times(uint32_t a, uint32_t c) {
+    uint32_t r;
+    if constexpr (BF) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0u), "r"(c));
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(0u), "r"(c));
+    return r;
+}
+// Stores of 32 bytes, a whole sector a lane.
+__device__ __forceinline__ void st32(void *p, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
 // A box of 64 columns from (x, y) of a tensor of 16-bit rows into the 128-byte swizzled layout.
 __device__ __forceinline__ void tma_box(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
@@ -189,9 +202,9 @@ template <int KIND, int D> struct TileUnit {
         t0 = int(max(lo - p.unit0, int64_t(0)));
         t1 = int(min(hi - p.unit0, int64_t(ntiles)));
         key_end = min(t1 * S::keys, q.keys(p.mt));
-        nrows = int(min(int64_t(S::rows), int64_t(unsigned(q.n) * unsigned(q.group) - unsigned(p.mt) * S::rows)));
+        nrows = int(min(int64_t(S::rows), int64_t(unsigned(q.n) * unsigned(io.group) - unsigned(p.mt) * S::rows)));
         // every row of the unit sees the keys below this
-        free_end = min(key_end, kv_seen(int(unsigned(p.mt) * S::rows / unsigned(q.group)), q.n, q.s.kv, q.causal));
+        free_end = min(key_end, kv_seen(int(by_group(io, unsigned(p.mt) * S::rows)), q.n, q.s.kv, io.causal));
     }
 };
 
@@ -270,8 +283,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     const int ur = w * 128 + r;
                     const bool live = ur < u.nrows;
                     const unsigned rr = unsigned(p.mt) * S::rows + ur;
-                    const int tok = int(rr / unsigned(u.q.group)), h = p.head * u.q.group + int(rr - unsigned(tok) * u.q.group);
-                    const int seen = live ? min(u.key_end, kv_seen(tok, u.q.n, u.q.s.kv, u.q.causal)) : 0;
+                    const int tok = int(by_group(io, rr)), h = p.head * io.group + int(rr - unsigned(tok) * io.group);
+                    const int seen = live ? min(u.key_end, kv_seen(tok, u.q.n, u.q.s.kv, io.causal)) : 0;
                     float fac = 0.0f;
                     float m = -INFINITY, l = 0.0f;
                     const uint32_t to = tmem + lanes + S::o_col + w * S::o_cols;
@@ -359,6 +372,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     fence_after();
                     const bool begun = p.unit0 < lo, unfinished = p.unit0 + u.ntiles > hi;
                     const bool dirty = *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) == unit;
+                    const bool wide = reinterpret_cast<uintptr_t>(io.out) % 32 == 0;
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                     float *part = AttnPart<S::rows, D>::slot(io.part, blockIdx.x, begun ? 0 : 1);
                     uint32_t *dst = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(io.out) +
@@ -386,9 +400,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         }
                         if (live && (begun || unfinished)) {
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                *reinterpret_cast<uint4 *>(part + ur * D + 32 * i + 4 * j) =
-                                    make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                            for (int j = 0; j < 4; ++j) st32(part + ur * D + 32 * i + 8 * j, v + 8 * j);
                         } else if (live) {
                             uint32_t y[16];
 #pragma unroll
@@ -396,10 +408,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                 const float e0 = __uint_as_float(v[2 * j]) * inv, e1 = __uint_as_float(v[2 * j + 1]) * inv;
                                 y[j] = io.q_bf16 ? pack_bf16(e0, e1) : pack_half(e0, e1);
                             }
+                            // (out is 16-byte aligned, 32 only where its allocation is)
+                            if (wide) {
+                                st32(dst + 16 * i, y);
+                                st32(dst + 16 * i + 8, y + 8);
+                            } else {
 #pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                *reinterpret_cast<uint4 *>(dst + 16 * i + 4 * j) =
-                                    make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                                for (int j = 0; j < 4; ++j)
+                                    *reinterpret_cast<uint4 *>(dst + 16 * i + 4 * j) =
+                                        make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                            }
                         }
                     }
                     if (live && (begun || unfinished)) {
@@ -451,7 +469,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const int all = (u.nrows > 128 ? S::rows : 128) * CHQ;
             auto row_at = [&](int ur) {
                 const unsigned rr = unsigned(p.mt) * S::rows + ur;
-                const int tok = int(rr / unsigned(u.q.group)), h = p.head * u.q.group + int(rr - unsigned(tok) * u.q.group);
+                const int tok = int(by_group(io, rr)), h = p.head * io.group + int(rr - unsigned(tok) * io.group);
                 return static_cast<const uint16_t *>(io.q) + (u.q.s.q0 + int64_t(tok)) * io.q_row + h * io.q_head;
             };
             auto place_q = [&](int ur, int ch) { return sq + (ch >> 3) * (S::rows * 128) + ur * 128 + (((ch & 7) ^ (ur & 7)) << 4); };
@@ -460,11 +478,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             // a negative scale: -q, so that the largest score stays the largest
             const uint32_t sign = io.scale_log2 < 0.0f ? 0x80008000u : 0;
             if (sign == 0 && !(S::quant && io.q_bf16)) {
-#pragma unroll 8
-                for (int at = qt; at < all; at += QT) {
-                    const int ur = at / CHQ, ch = at % CHQ;
+                const int ch = qt % CHQ;  // of every row of this thread
+#pragma unroll 4
+                for (int ur = qt / CHQ; ur < all / CHQ; ur += QT / CHQ) {
+                    const bool live = ur < u.nrows;
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(place_q(ur, ch))),
-                                 "l"(ur < u.nrows ? row_at(ur) + ch * 8 : io.q), "r"(ur < u.nrows ? 16 : 0)
+                                 "l"(live ? row_at(ur) + ch * 8 : io.q), "r"(live ? 16 : 0)
                                  : "memory");
                     if (ch == 0) put_fac(ur, 0);
                 }
@@ -518,18 +537,27 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             auto clean = [&](const TileUnit<KIND, D> &u, int t, int b, int from) {  // by threads `from` and up
                 const int left = u.key_end - t * S::keys;
                 const uint32_t bad[2] = {sh.bad[seq & 7][0], sh.bad[seq & 7][1]};
-#pragma unroll 2
-                for (int at = tid - from; at < S::keys * CH; at += LT - from) {
-                    const int r = at / CH;
-                    uint4 *w4 = reinterpret_cast<uint4 *>(place(1, b, r, at % CH));
-                    const uint4 x = *w4;
-                    const uint32_t n[4] = {nonfinite2<BF>(x.x), nonfinite2<BF>(x.y), nonfinite2<BF>(x.z), nonfinite2<BF>(x.w)};
-                    if (r >= left || ((bad[r >> 5] >> (r & 31)) & 1)) {
-                        *w4 = make_uint4(0, 0, 0, 0);
-                    } else if (n[0] | n[1] | n[2] | n[3]) {
-                        *w4 = make_uint4(x.x & ~n[0], x.y & ~n[1], x.z & ~n[2], x.w & ~n[3]);
-                        *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
+                const int step = (LT - from) / CH, ch = (tid - from) % CH, first = (tid - from) / CH;
+                if (left < S::keys || (bad[0] | bad[1])) {
+                    for (int r = first; r < S::keys; r += step)
+                        if (r >= left || ((bad[r >> 5] >> (r & 31)) & 1))
+                            *reinterpret_cast<uint4 *>(place(1, b, r, ch)) = make_uint4(0, 0, 0, 0);
+                }
+                // 0 x value summed: NaN if any value is not finite
+                uint32_t odd = 0;
+#pragma unroll 4
+                for (int r = first; r < S::keys; r += step) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(place(1, b, r, ch));
+                    odd = zero_times<BF>(x.x, zero_times<BF>(x.y, zero_times<BF>(x.z, zero_times<BF>(x.w, odd))));
+                }
+                if (nonfinite2<BF>(odd)) {
+                    for (int r = first; r < S::keys; r += step) {
+                        uint4 *w4 = reinterpret_cast<uint4 *>(place(1, b, r, ch));
+                        const uint4 x = *w4;
+                        *w4 = make_uint4(x.x & ~nonfinite2<BF>(x.x), x.y & ~nonfinite2<BF>(x.y), x.z & ~nonfinite2<BF>(x.z),
+                                         x.w & ~nonfinite2<BF>(x.w));
                     }
+                    *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) = unit;
                 }
                 __syncwarp();
             };
