@@ -51,7 +51,7 @@ static AttnPlan attn_plan(const anvil_kv_cache *c, const KvCacheView &cv, const 
     const int64_t slots = 148 * t.occ;
     p.ctas = int(per > slots / std::max<int64_t>(units, 1) ? slots : std::min(slots, units * per));
     p.join = per > 1;
-    p.bytes = p.join ? int64_t(t.rows) * (c->head_dim + 2) * 8 * p.ctas : 0;
+    p.bytes = p.join ? (int64_t(t.rows) * (c->head_dim + 2) * 8 + int64_t(sizeof(AttnOpen))) * p.ctas : 0;
     return p;
 }
 

@@ -8,7 +8,7 @@
 // every CTA has the same work whatever the lengths, and neighbouring CTAs read the same keys.  A
 // unit that lies in one share is finished there; a unit that spans shares leaves one partial
 // result (unnormalised output, maximum, sum) per share, and a second kernel joins them in the
-// order of the shares, so results do not depend on timing.  Lengths are read on the device; the
+// order of the shares, so results do not depend on timing; it is told which units by a note of each CTA.  Lengths are read on the device; the
 // grid depends on the batch's outer sizes alone, so a captured graph replays with other lengths.
 #pragma once
 
@@ -57,6 +57,16 @@ template <int ROWS, int D> struct AttnPart {
         return part + (int64_t(cta) * 2 + which) * floats;
     }
 };
+
+// What CTA c says of slot 2 c + 1, behind all slots: the unit it began and did not finish.
+struct alignas(16) AttnOpen {
+    int parts;               // CTAs that have a part of it, c and the next ones; 0: none
+    int token0, head0, row0; // its sequence's first packed row, its first query head, its first row
+    int rows, pad[3];        // rows of the unit
+};
+template <int ROWS, int D> __device__ __forceinline__ AttnOpen *attn_open(float *part, int ctas) {
+    return reinterpret_cast<AttnOpen *>(AttnPart<ROWS, D>::slot(part, ctas, 0));
+}
 
 // One sequence's units: row tiles and their key tiles.  Rows are counted in 32 bits (the host refuses
 // batches of 2^31 query rows).
@@ -352,29 +362,19 @@ __device__ __forceinline__ uint32_t dup16(uint32_t x) { return __byte_perm(x, x,
 // not finish: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.  A row's parts are shared by 1, 2, 4 or 8 of the
 // eight warps, at most 8 parts a warp where there are that many; the order of the sums is fixed by the parts.
 constexpr int kJoinWarps = 8;
-template <int ROWS, int KEYS, int COST, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(KvCacheView c, KvBatchView bt, AttnIO io) {
-    __shared__ AttnScratch sc;
+template <int ROWS, int D>
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(AttnIO io) {
     __shared__ __align__(16) float so[kJoinWarps][D];
     __shared__ float sl[kJoinWarps];
     const int cta = blockIdx.x;
-    const int64_t work = attn_locate<ROWS, KEYS, COST>(
-        c, bt, io, &sc, [&](const AttnShares &s) { return s.begin(min(cta + 1, s.ctas)) - 1; },  // the share's last place
-        false);
     pdl_wait();  // the partial results are the kernel before's; waited for by every CTA
-    const AttnShares shares(work, gridDim.x);
-    if (cta >= shares.ctas) return;
-    const AttnPos p = sc.pos;
-    const int64_t lo = shares.begin(cta), hi = shares.begin(cta + 1);
-    if (p.unit0 < lo || p.unit0 >= hi) return;  // begun elsewhere
-    const AttnSeq<ROWS, KEYS> q(load_seq(bt, c, p.b), io);
-    const int64_t end = p.unit0 + q.key_tiles(p.mt);
-    if (end <= hi) return;  // finished where it was begun
-    const int np = shares.owner(end - 1) - cta + 1;
+    const AttnOpen open = attn_open<ROWS, D>(io.part, gridDim.x)[cta];
+    const int np = open.parts;
+    if (np == 0) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int share = np > 32 ? 8 : np > 16 ? 4 : np > 8 ? 2 : 1;  // warps of a row
     const int sub = warp % share, rows = kJoinWarps / share;        // rows at once
-    const int nrows = int(min(unsigned(ROWS), unsigned(q.n) * unsigned(io.group) - unsigned(p.mt) * ROWS));
+    const int nrows = open.rows;
     using P = AttnPart<ROWS, D>;
     constexpr int V = D / 32;
     for (int r0 = blockIdx.y * rows; r0 < nrows; r0 += rows * gridDim.y) {
@@ -431,8 +431,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(KvCacheView 
         }
         if (!live || sub) continue;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const unsigned r = unsigned(p.mt) * ROWS + row;
-        const int tok = int(by_group(io, r)), token = q.s.q0 + tok, h = p.head * io.group + int(r - unsigned(tok) * io.group);
+        const unsigned r = unsigned(open.row0) + row;
+        const int tok = int(by_group(io, r)), token = open.token0 + tok, h = open.head0 + int(r - unsigned(tok) * io.group);
         uint32_t *out = reinterpret_cast<uint32_t *>(static_cast<uint16_t *>(io.out) +
                                                      (int64_t(token) * io.heads + h) * D) + lane * (V / 2);
 #pragma unroll
@@ -447,11 +447,9 @@ struct AttnTiles {
     int rows, keys, occ;
 };
 
-template <int ROWS, int KEYS, int COST, int D>
-static int attn_join_launch(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
-                            cudaStream_t stream) {
+template <int ROWS, int D> static int attn_join_launch(const AttnIO &io, int ctas, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, std::min(ROWS / 4, 8));
+    cfg.gridDim = dim3(ctas, std::min(ROWS / 2, 8));
     cfg.blockDim = kJoinWarps * 32;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -459,7 +457,7 @@ static int attn_join_launch(const KvCacheView &c, const KvBatchView &bt, const A
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_join_kernel<ROWS, KEYS, COST, D>, c, bt, io);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_join_kernel<ROWS, D>, io);
     return e == cudaSuccess ? ANVIL_OK : cuda_fail(e, "paged_attention join launch");
 }
 

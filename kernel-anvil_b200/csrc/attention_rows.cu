@@ -2,8 +2,8 @@
 // cache: row tiles of 8 or 16, bound by the bytes of the cache.
 //
 // Arithmetic: mma.sync m16n8k16 with fp32 sums, transposed so that the keys, not the few queries,
-// fill the 16 rows of a product: S^T = K Q^T (16 keys x 8 queries), then the running maximum and
-// sum, then O^T += V^T P^T with P rounded to the products' 16-bit type.  A tile of 8 queries costs
+// fill the 16 rows of a product: S^T = K Q^T (16 keys x 8 queries), then the weights by a reference that
+// is raised when one grows large, and their sum, then O^T += V^T P^T with P rounded to the products' 16-bit type.  A tile of 8 queries costs
 // half the products, exponentials and registers that a 16-row tile of queries would, and widening
 // the codes, which dominates, is done once for all queries.  The legacy tensor path is enough:
 // it works a fifth of the time at the rate at which HBM delivers keys, and tcgen05's smallest tile
@@ -32,6 +32,7 @@ namespace anvil {
 constexpr int kRowsWarps = 4;
 constexpr int kRowsStep = 16;   // keys of a warp's step
 constexpr int kRowsKeys = 64;   // keys of a key tile: one step of each warp
+constexpr float kRowsSlack = 16384.0f;  // the largest weight
 constexpr int kRowsCost = 0;    // beginning and ending a unit, in key tiles
 
 template <int KIND, int D, int NT> struct RowsShape {
@@ -45,7 +46,7 @@ template <int KIND, int D, int NT> struct RowsShape {
     static constexpr int off_bad = off_s + 2 * kRowsStep * sb;
     static constexpr int stage = off_bad + 16;
     // two stages keep 16 keys of every warp in flight while 16 are worked on; short rows take more
-    static constexpr int stages = stage <= 2800 ? 4 : stage <= 5200 ? 3 : 2;
+    static constexpr int stages = stage <= 1400 ? 4 : stage <= 2800 ? 3 : 2;
     static constexpr int ring = stage * stages;             // of one warp
     static constexpr int join = rows * (D + 4) * 4 + rows * 8;  // of one warp, reuses the ring
     static constexpr int per_warp = ((ring > join ? ring : join) + 15) & ~15;
@@ -140,6 +141,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
         c, bt, io, &sc, [&](const AttnShares &s) { return s.begin(min(int(blockIdx.x), s.ctas - 1)); }, blockIdx.x == 0);
     pdl_launch_dependents();
     const AttnShares shares(work, gridDim.x);
+    // what is to be joined: nothing, unless the last unit is left unfinished below
+    if (io.part && threadIdx.x == 0) attn_open<ROWS, D>(io.part, gridDim.x)[blockIdx.x].parts = 0;
     if (int(blockIdx.x) >= shares.ctas) return;
     const int64_t lo = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
     AttnPos p = sc.pos;
@@ -268,7 +271,14 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                     qb[t][s][0] = __byte_perm(x, y, 0x5410);
                     qb[t][s][1] = __byte_perm(x, y, 0x7632);
                 }
-            const float my_fac = io.scale_log2 * pow2i(-ex);
+            // A negative scale: -q, so that the largest score stays the largest.  Above zero, so that a masked score stays -inf.
+            if (io.scale_log2 < 0.0f)
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    qb[t][s][0] ^= 0x80008000u;
+                    qb[t][s][1] ^= 0x80008000u;
+                }
+            const float my_fac = fmaxf(fabsf(io.scale_log2) * pow2i(-ex), 1e-36f);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 seen[t][e] = min(__shfl_sync(0xffffffffu, my_seen, (2 * cq + e) * 4), key_end);
@@ -278,7 +288,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
         // every row of the unit sees the keys below this: no mask is needed there
         const int free_end = min(key_end, kv_seen(int(by_group(io, unsigned(p.mt) * ROWS)), q.n, q.s.kv, io.causal));
 
-        float o[NT][MT][4], m[NT][2], l[NT][2];
+        // m: references; nb: their negatives, 0 for none; fresh: some row has none
+        float o[NT][MT][4], m[NT][2], l[NT][2], nb[NT][2];
+        bool fresh = true;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -286,7 +298,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[t][i][j] = 0.0f;
             m[t][0] = m[t][1] = -INFINITY;
-            l[t][0] = l[t][1] = 0.0f;
+            l[t][0] = l[t][1] = nb[t][0] = nb[t][1] = 0.0f;
         }
 
         for (int s = step0; s < steps; s += 4) {
@@ -357,13 +369,10 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                 }
             }
 
-            // ---- scores, running maximum and sum
+            // ---- weights by the rows' references m.  Only where one exceeds 2^14 (fp16 ends at 65504), or where there is
+            // no reference yet, is the step's maximum looked for, made the reference, and the step taken again.
             const int key0 = s * kRowsStep;
             const bool masked = key0 + kRowsStep > free_end || bad != 0;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sc2[t][j] *= fac[t][j & 1];
             if (masked) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
@@ -373,41 +382,45 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                         if (key0 + k >= seen[t][j & 1] || ((bad >> k) & 1)) sc2[t][j] = -INFINITY;
                     }
             }
-            float mn[NT][2], base[NT][2];
-            bool grew = false;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float x = fmaxf(sc2[t][e], sc2[t][2 + e]);
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    mn[t][e] = fmaxf(m[t][e], x);
-                    base[t][e] = mn[t][e] == -INFINITY ? 0.0f : mn[t][e];
-                    grew |= mn[t][e] > m[t][e];
-                }
-            if (__any_sync(0xffffffffu, grew)) {
+            uint32_t pb[NT][2];
+            float e[NT][4];
+            for (bool first = true;; first = false) {
+                bool raise = false;
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float a = ex2(m[t][e] - base[t][e]);
-                        l[t][e] *= a;
-                        m[t][e] = mn[t][e];
+                    for (int j = 0; j < 4; ++j) {
+                        e[t][j] = ex2(fmaf(sc2[t][j], fac[t][j & 1], nb[t][j & 1]));
+                        raise |= e[t][j] > kRowsSlack;
+                    }
+                if (!__any_sync(0xffffffffu, (raise || fresh) && first)) break;
+                fresh = false;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) {
+                        float x = fmaxf(sc2[t][d], sc2[t][2 + d]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * fac[t][d];
+                        const float mn = fmaxf(m[t][d], x);
+                        const float a = mn == -INFINITY ? 1.0f : ex2(m[t][d] - mn);
+                        fresh |= mn == -INFINITY;  // a row without keys so far
+                        l[t][d] *= a;
+                        m[t][d] = mn;
+                        nb[t][d] = mn == -INFINITY ? 0.0f : -mn;
 #pragma unroll
                         for (int i = 0; i < MT; ++i) {
-                            o[t][i][e] *= a;
-                            o[t][i][2 + e] *= a;
+                            o[t][i][d] *= a;
+                            o[t][i][2 + d] *= a;
                         }
                     }
             }
-            uint32_t pb[NT][2];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const float x = ex2(sc2[t][2 * i] - base[t][0]), y = ex2(sc2[t][2 * i + 1] - base[t][1]);
+                    const float x = e[t][2 * i], y = e[t][2 * i + 1];
                     l[t][0] += x;
                     l[t][1] += y;
                     pb[t][i] = transpose8(BF ? pack_bf16(x, y) : pack_half(x, y));
@@ -580,6 +593,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
         __syncthreads();
         const bool begun = p.unit0 < lo, unfinished = p.unit0 + ntiles > hi;
         float *part = AttnPart<ROWS, D>::slot(io.part, blockIdx.x, begun ? 0 : 1);
+        if (unfinished && !begun && threadIdx.x == 0)
+            attn_open<ROWS, D>(io.part, gridDim.x)[blockIdx.x] =
+                AttnOpen{shares.owner(p.unit0 + ntiles - 1) - int(blockIdx.x) + 1, q.s.q0, p.head * io.group, p.mt * ROWS, nrows, {}};
         for (int r = warp; r < nrows; r += kRowsWarps) {
             float mw[kRowsWarps], mx = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -639,7 +655,7 @@ template <int KIND, int D, int NT> struct RowsOps {
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
         attn_rows_kernel<KIND, D, NT><<<ctas, kRowsWarps * 32, S::smem, stream>>>(c, bt, io);
         if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "paged_attention launch");
-        return join ? attn_join_launch<S::rows, kRowsKeys, kRowsCost, D>(c, bt, io, ctas, stream) : ANVIL_OK;
+        return join ? attn_join_launch<S::rows, D>(io, ctas, stream) : ANVIL_OK;
     }
 };
 

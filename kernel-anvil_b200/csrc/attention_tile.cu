@@ -224,7 +224,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         c, bt, io, &sh.sc, [&](const AttnShares &s) { return s.begin(min(int(blockIdx.x), s.ctas - 1)); }, blockIdx.x == 0);
     pdl_launch_dependents();
     const AttnShares shares(work, gridDim.x);
-    if (int(blockIdx.x) >= shares.ctas) return;
+    AttnOpen *const note = io.part ? attn_open<S::rows, D>(io.part, gridDim.x) + blockIdx.x : nullptr;
+    if (int(blockIdx.x) >= shares.ctas) {
+        if (note && threadIdx.x == 0) *note = AttnOpen{};
+        return;
+    }
     const int64_t lo = shares.begin(blockIdx.x), hi = shares.begin(blockIdx.x + 1);
     AttnPos p = sh.sc.pos;
     KvSeq kseq = load_seq(bt, c, p.b);
@@ -275,6 +279,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // ahead of the other, and a parity tells one phase from the next only.
         uint32_t n0 = 0, n1 = 0;
         int unit = 0, seq = 0;              // units and key tiles so far, counted alike in every role
+        bool noted = false;
         if (w < S::nq)
             while (p.b < bt.batch && p.unit0 < hi) {
                 const TileUnit<KIND, D> u(kseq, io, p, lo, hi);
@@ -371,6 +376,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     __syncwarp();
                     fence_after();
                     const bool begun = p.unit0 < lo, unfinished = p.unit0 + u.ntiles > hi;
+                    if (unfinished && !begun && threadIdx.x == 0) {
+                        noted = true;
+                        *note = AttnOpen{shares.owner(p.unit0 + u.ntiles - 1) - int(blockIdx.x) + 1, u.q.s.q0, p.head * io.group, p.mt * S::rows, u.nrows, {}};
+                    }
                     const bool dirty = *reinterpret_cast<volatile int *>(&sh.dirty[unit & 7]) == unit;
                     const bool wide = reinterpret_cast<uintptr_t>(io.out) % 32 == 0;
                     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -429,6 +438,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 seq += u.t1 - u.t0;
                 attn_next<S::rows, S::keys, kTileCost>(c, bt, io, p, kseq);
             }
+        if (threadIdx.x == 0 && note && !noted) *note = AttnOpen{};
     } else if (warp < 12) {
         // ================= loaders: keys and values of a tile together ===============================
         constexpr int LT = kTileLoaders;
@@ -1003,7 +1013,7 @@ template <int KIND, int D> static int launch_tile(const KvCacheView &c, const Kv
     }
     attn_tile_kernel<KIND, D><<<ctas, kTileThreads, S::smem, stream>>>(c, bt, io, mk, mv, box, wait_limit_ns());
     if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "paged_attention launch");
-    return join ? attn_join_launch<S::rows, S::keys, kTileCost, D>(c, bt, io, ctas, stream) : ANVIL_OK;
+    return join ? attn_join_launch<S::rows, D>(io, ctas, stream) : ANVIL_OK;
 }
 
 template <int KIND> static int tile_dim(int D, const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
