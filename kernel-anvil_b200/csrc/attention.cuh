@@ -15,6 +15,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "anvil.h"
 #include "anvil_host.h"
@@ -440,6 +441,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(AttnIO io) {
             out[j] = io.q_bf16 ? pack_bf16(o[2 * j] * inv, o[2 * j + 1] * inv)
                                : pack_half(o[2 * j] * inv, o[2 * j + 1] * inv);
     }
+}
+
+// Lets `fn` use `bytes` of dynamic shared memory, once for each device (up to 64; beyond, every time).
+template <typename F> static cudaError_t attn_allow_smem(F *fn, int bytes, std::atomic<uint64_t> *done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done->load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done->fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // Host side: a kernel's row tile, key tile and resident CTAs of an SM.

@@ -650,8 +650,8 @@ template <int KIND, int D, int NT> struct RowsOps {
     using S = RowsShape<KIND, D, NT>;
     static int launch(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas, bool join,
                       cudaStream_t stream) {
-        cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<KIND, D, NT>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+        static std::atomic<uint64_t> allowed{0};
+        cudaError_t e = attn_allow_smem(attn_rows_kernel<KIND, D, NT>, S::smem, &allowed);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
         attn_rows_kernel<KIND, D, NT><<<ctas, kRowsWarps * 32, S::smem, stream>>>(c, bt, io);
         if ((e = cudaGetLastError()) != cudaSuccess) return cuda_fail(e, "paged_attention launch");

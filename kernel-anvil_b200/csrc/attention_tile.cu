@@ -994,7 +994,8 @@ static int tile_map(CUtensorMap *map, void *data, int D, int64_t rows, int box) 
 template <int KIND, int D> static int launch_tile(const KvCacheView &c, const KvBatchView &bt, const AttnIO &io, int ctas,
                                                   bool join, cudaStream_t stream) {
     using S = TileShape<KIND, D>;
-    cudaError_t e = cudaFuncSetAttribute(attn_tile_kernel<KIND, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t e = attn_allow_smem(attn_tile_kernel<KIND, D>, S::smem, &allowed);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
     // The warp groups' shares of the registers add up to 128 a thread: a build with fewer must not be launched
     // (the group that asks for more would wait for ever).

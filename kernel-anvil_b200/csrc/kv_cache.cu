@@ -113,6 +113,22 @@ __device__ __forceinline__ uint32_t block_amax_bits(const float (&x)[8]) {
 
 __device__ __forceinline__ float clamp_kv(float x) { return fminf(fmaxf(x, -kKvMax), kKvMax); }
 
+// The fast paths below compute a value's code in five fp32 operations and no branch, with a flag for the values
+// that lie near a border between two codes; the exact functions then decide (one block of 8 in 600 does,
+// for random values).  Taken for every value, they made the write of 8000 tokens take 25 us instead of FILLQ8.
+constexpr float kKvMagic = 12582912.0f;  // 1.5 * 2^23: x + kKvMagic holds round(x) in its last bits
+constexpr float kKvNear = 0.4999f;       // |x - round(x)| from here on: near a border
+
+// fp16(M / 127) where the product with 1 / 127 (off by 2 units in the last place at most) is not near a border
+// between two halves; else and for subnormal halves, exactly.
+__device__ __forceinline__ __half q8_scale_half(float M);
+__device__ __forceinline__ __half q8_scale_fast(float M) {
+    const float q = M * (1.0f / 127.0f);
+    const uint32_t rest = __float_as_uint(q) & 0x1FFFu;
+    if (q < 0x1p-13f || (rest > 0x1000u - 8 && rest < 0x1000u + 8)) return q8_scale_half(M);
+    return __float2half_rn(q);
+}
+
 // fp16(M / 127), rounded once: the truncated quotient with a sticky last bit (set when the
 // remainder M - q 127, which fma gives exactly, is not zero) rounds to fp16 as M / 127 does.
 __device__ __forceinline__ __half q8_scale_half(float M) {
@@ -142,8 +158,24 @@ __device__ __forceinline__ uint2 quant8_q8(const float (&x)[8], __half &d) {
         return w;
     }
     const float M = fminf(__uint_as_float(mb), kKvMax);
-    d = q8_scale_half(M);
+    d = q8_scale_fast(M);
     if (M == 0.0f) return w;
+    if (M >= 0x1p-100f && M < kKvMax) {
+        const float inv = __fdividef(127.0f, M);  // 127 |x| / M off by less than 1e-4
+        float far = 0.0f;
+        uint32_t r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float t = x[i] * inv, m = t + kKvMagic;
+            far = fmaxf(far, fabsf(t - (m - kKvMagic)));
+            r[i] = __float_as_uint(m);
+        }
+        if (far < kKvNear) {
+            w.x = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+            w.y = __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410);
+            return w;
+        }
+    }
     // below 2^-100 M is scaled up with its block (exactly), so that no quotient or remainder
     // is subnormal; such a block's scale is zero in fp16 and its codes stand for zeros
     const float up = M < 0x1p-100f ? 0x1p100f : 1.0f;
@@ -195,9 +227,21 @@ __device__ __forceinline__ uint32_t quant8_q4(const float (&x)[8], __half &d) {
         d = __float2half_rn(0.0f);
         return 0x88888888u;
     }
+    uint32_t w = 0;  // nibble i = value i
+    if (M >= 0x1p-100f && M < kKvMax) {
+        const float inv = __fdividef(-8.0f, top);
+        float far = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float t = x[i] * inv, m = fminf(t, 7.25f) + (kKvMagic + 8.0f);  // (code 15 is the last)
+            far = fmaxf(far, t > 7.25f ? 0.0f : fabsf(t - (m - (kKvMagic + 8.0f))));
+            w |= (__float_as_uint(m) & 15u) << (4 * i);
+        }
+        if (far < kKvNear) return w;
+        w = 0;
+    }
     const float up = M < 0x1p-100f ? 0x1p100f : 1.0f;
     const float ts = top * up, inv = -8.0f / ts;
-    uint32_t w = 0;  // nibble i = value i
 #pragma unroll
     for (int i = 0; i < 8; ++i) w |= uint32_t(q4_code(clamp_kv(x[i]) * up, ts, inv)) << (4 * i);
     return w;

@@ -114,6 +114,7 @@ class PagedKVCache:
         self._c = _Cache(ggml, pages, heads, size, dim, k.data_ptr(), v.data_ptr(),
                          k_scale.data_ptr() if per else None, v_scale.data_ptr() if per else None)
         self._ref = ctypes.byref(self._c)
+        self._work: dict[tuple, int] = {}  # attention scratch by (batch, rows, pages, heads): it depends on these alone
 
     @property
     def bytes_per_token(self) -> int:
@@ -131,52 +132,67 @@ _INT = torch.int32
 
 
 def _batch(cache: PagedKVCache, page_table, start, kv_len, total: int) -> _Batch:
-    if not cache.k.is_cuda:
-        raise _bad("the cache must be on a CUDA device (no CPU path)")
-    n = start.shape[0] - 1
-    if start.dtype != _INT or start.dim() != 1 or n < 0 or not start.is_contiguous():
-        raise _bad("the starts are a contiguous int32 tensor of batch + 1 values")
-    if page_table.dtype != _INT or page_table.dim() != 2 or page_table.shape[0] != n or \
-            (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise _bad(f"page_table is an int32 tensor ({n}, pages) with contiguous rows")
-    if kv_len is not None and (kv_len.dtype != _INT or kv_len.shape != (n,) or not kv_len.is_contiguous()):
-        raise _bad(f"kv_len is a contiguous int32 tensor of {n} values")
     dev = cache.device
-    if start.device != dev or page_table.device != dev or (kv_len is not None and kv_len.device != dev):
-        raise _bad("page_table, starts and kv_len must be on the cache's device")
+    if dev.type != "cuda":
+        raise _bad("the cache must be on a CUDA device (no CPU path)")
+    shape = start.shape
+    if len(shape) != 1 or shape[0] < 1 or start.dtype != _INT or not start.is_contiguous():
+        raise _bad("the starts are a contiguous int32 tensor of batch + 1 values")
+    n = shape[0] - 1
+    shape = page_table.shape
+    if len(shape) != 2 or shape[0] != n or page_table.dtype != _INT:
+        raise _bad(f"page_table is an int32 tensor ({n}, pages) with contiguous rows")
+    pages = shape[1]
+    step, inner = page_table.stride()
+    if pages > 1 and inner != 1:
+        raise _bad(f"page_table is an int32 tensor ({n}, pages) with contiguous rows")
+    if start.device != dev or page_table.device != dev:
+        raise _bad("page_table, starts and lengths must be on the cache's device")
+    lens = None
+    if kv_len is not None:
+        if kv_len.dtype != _INT or kv_len.shape != (n,) or not kv_len.is_contiguous():
+            raise _bad(f"lengths and first positions are contiguous int32 tensors of {n} values")
+        if kv_len.device != dev:
+            raise _bad("page_table, starts and lengths must be on the cache's device")
+        lens = kv_len.data_ptr()
     if total > 0x7FFFFFFF:
         raise _bad("more than 2^31 - 1 rows in one call")
-    pages = page_table.shape[1]
-    return _Batch(page_table.data_ptr(), page_table.stride(0) if n > 1 else pages, pages, n, total,
-                  start.data_ptr(), kv_len.data_ptr() if kv_len is not None else None)
+    return _Batch(page_table.data_ptr(), step if n > 1 else pages, pages, n, total, start.data_ptr(), lens)
 
 
 def _rows(name: str, x: torch.Tensor, cache: PagedKVCache, heads: int | None) -> torch.Tensor:
     """x as (rows, heads, head_dim) whose rows start on 16-byte boundaries (copied where they do not)."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if x.dim() != 3 or x.shape[2] != cache.head_dim or (heads is not None and x.shape[1] != heads):
-        raise _bad(f"{name} is (rows, {heads or 'heads'}, {cache.head_dim}), got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != cache.head_dim or (heads is not None and shape[1] != heads):
+        raise _bad(f"{name} is (rows, {heads or 'heads'}, {cache.head_dim}), got {tuple(shape)}")
     if x.device != cache.device:
         raise _bad(f"{name} must be on the cache's device {cache.device}, got {x.device}")
     if x.dtype not in DTYPES:
         raise _bad(f"{name} must be float32, float16 or bfloat16, got {x.dtype}")
     if x.requires_grad and torch.is_grad_enabled():
         raise _bad(f"{name} requires grad, and the cache's operators have no backward pass")
-    n = 16 // x.element_size()
-    if x.stride(2) != 1 or x.stride(0) % n or x.stride(1) % n or x.data_ptr() % 16:
+    row, head, inner = x.stride()
+    n = 4 if x.dtype == torch.float32 else 8  # values in 16 bytes
+    if inner != 1 or row % n or head % n or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
+
+
+_stream = torch._C._cuda_getCurrentRawStream  # of a device index, without the Stream object
 
 
 def _call(cache: PagedKVCache, fn, *args) -> None:
     """fn(*args, stream) on the cache's device and torch's current stream there."""
     index = cache.device.index
-    if index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream(index).cuda_stream))
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, _stream(index))
     else:
         with torch.cuda.device(index):
-            check(fn(*args, torch.cuda.current_stream(index).cuda_stream))
+            status = fn(*args, _stream(index))
+    if status < 0:
+        check(status)
 
 
 def kv_write(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
@@ -249,7 +265,13 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     if kv_len is None:
         raise _bad("kv_len is needed")
     lib, ref = _native.lib(), ctypes.byref(b)
-    need = check(lib.anvil_paged_attention_workspace(cache._ref, ref, heads))
+    key = (b.batch, b.total, b.max_pages, heads)
+    need = cache._work.get(key)
+    if need is None:
+        need = check(lib.anvil_paged_attention_workspace(cache._ref, ref, heads))
+        if len(cache._work) > 4096:  # ragged totals of a long-lived server
+            cache._work.clear()
+        cache._work[key] = need
     # scratch of this call, from torch's allocator: its memory follows the stream and, in a capture, the graph
     work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
     _call(cache, lib.anvil_paged_attention, cache._ref, ref, DTYPES[q.dtype], q.data_ptr(), q.stride(0),
