@@ -106,16 +106,17 @@ template <> struct Vec8<__nv_bfloat16> {
 __device__ __forceinline__ uint32_t block_amax_bits(const float (&x)[8]) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    for (int i = 0; i < 8; i += 2)
+        m = __vimax3_u32(m, __float_as_uint(x[i]) & 0x7FFFFFFFu, __float_as_uint(x[i + 1]) & 0x7FFFFFFFu);
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
 }
 
 __device__ __forceinline__ float clamp_kv(float x) { return fminf(fmaxf(x, -kKvMax), kKvMax); }
 
-// The fast paths below compute a value's code in five fp32 operations and no branch, with a flag for the values
-// that lie near a border between two codes; the exact functions then decide (one block of 8 in 600 does,
-// for random values).  Taken for every value, they made the write of 8000 tokens take 25 us instead of FILLQ8.
+// A value's code takes five fp32 operations; one that lies near a border between two codes is then decided
+// exactly.  (With the exact decision inlined for every value the write of 8000 tokens took 30 us; inputs of 16
+// bits lie on borders of Q4_0 often, so that recomputing a lane's eight values for one of them was no better.)
 constexpr float kKvMagic = 12582912.0f;  // 1.5 * 2^23: x + kKvMagic holds round(x) in its last bits
 constexpr float kKvNear = 0.4999f;       // |x - round(x)| from here on: near a border
 
@@ -137,17 +138,13 @@ __device__ __forceinline__ __half q8_scale_half(float M) {
     return __float2half_rn(__uint_as_float(__float_as_uint(q) | sticky));
 }
 
-// round_half_away(127 a / M) for 0 <= a <= M: the candidate is off by one at most where
-// 127 a / M is within 1e-4 of a border k + 1/2; there the sign of 127 a - (k + 1/2) M decides.
-// p + e is 127 a exactly, and p - (k + 1/2) M is exact this near to zero.
-__device__ __forceinline__ int q8_code(float a, float M, float inv) {
-    const float t = a * inv;
-    const float k = floorf(t);
-    const float f = t - k;
-    if (fabsf(f - 0.5f) > 1e-4f) return int(k) + (f > 0.5f ? 1 : 0);
+// round_half_away(127 x / M) where t = 127 x / M to within 1e-4 and k = round(t) are known and t lies near a border
+// of k, b = |k| +- 1/2: the sign of 127 |x| - b M decides.  p + e is 127 |x| exactly, and p - b M is exact this near
+// to zero.
+__device__ __noinline__ float q8_border(float x, float M, float t, float k) {
+    const float a = fabsf(x), b = fabsf(k) + (fabsf(t) > fabsf(k) ? 0.5f : -0.5f);
     const float p = a * 127.0f, e = fmaf(a, 127.0f, -p);
-    const float r = fmaf(-(k + 0.5f), M, p) + e;
-    return int(k) + (r >= 0.0f ? 1 : 0);
+    return copysignf(b + (fmaf(-b, M, p) + e >= 0.0f ? 0.5f : -0.5f), x);
 }
 
 __device__ __forceinline__ uint2 quant8_q8(const float (&x)[8], __half &d) {
@@ -160,51 +157,27 @@ __device__ __forceinline__ uint2 quant8_q8(const float (&x)[8], __half &d) {
     const float M = fminf(__uint_as_float(mb), kKvMax);
     d = q8_scale_fast(M);
     if (M == 0.0f) return w;
-    if (M >= 0x1p-100f && M < kKvMax) {
-        const float inv = __fdividef(127.0f, M);  // 127 |x| / M off by less than 1e-4
-        float far = 0.0f;
-        uint32_t r[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float t = x[i] * inv, m = t + kKvMagic;
-            far = fmaxf(far, fabsf(t - (m - kKvMagic)));
-            r[i] = __float_as_uint(m);
-        }
-        if (far < kKvNear) {
-            w.x = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
-            w.y = __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410);
-            return w;
-        }
-    }
     // below 2^-100 M is scaled up with its block (exactly), so that no quotient or remainder
     // is subnormal; such a block's scale is zero in fp16 and its codes stand for zeros
-    const float up = M < 0x1p-100f ? 0x1p100f : 1.0f;
-    const float Ms = M * up, inv = 127.0f / Ms;
-    uint32_t u[2] = {0, 0};
+    const float up = M < 0x1p-100f ? 0x1p100f : 1.0f, Ms = M * up;
+    const float inv = __fdividef(127.0f, Ms);  // 127 x / M off by less than 1e-4
+    uint32_t r[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float c = clamp_kv(x[i]) * up;
-        const int q = q8_code(fabsf(c), Ms, inv);
-        u[i >> 2] |= (uint32_t(c < 0 ? -q : q) & 0xFFu) << (8 * (i & 3));
+        const float c = clamp_kv(x[i]) * up, t = c * inv, m = t + kKvMagic, k = m - kKvMagic;
+        r[i] = __float_as_uint(m);
+        if (fabsf(t - k) >= kKvNear) r[i] = __float_as_uint(q8_border(c, Ms, t, k) + kKvMagic);
     }
-    w.x = u[0];
-    w.y = u[1];
+    w.x = __byte_perm(__byte_perm(r[0], r[1], 0x0040), __byte_perm(r[2], r[3], 0x0040), 0x5410);
+    w.y = __byte_perm(__byte_perm(r[4], r[5], 0x0040), __byte_perm(r[6], r[7], 0x0040), 0x5410);
     return w;
 }
 
-// Nibble of value x for the block's top value: floor(x / d + 8.5) with d = top / -8 is
-// 8 + round of -8 x / top, halves upwards, cut to 0..15; a border n + 1/2 is decided by the sign of
-// |16 x| - |2 n + 1| |top|, exact in one fma.
-__device__ __forceinline__ int q4_code(float x, float top, float inv) {
-    const float t = x * inv;  // -8 x / top, within [-8, 8]
-    const float k = floorf(t), f = t - k;
-    int q = int(k) + (f >= 0.5f ? 1 : 0);
-    if (fabsf(f - 0.5f) <= 1e-5f) {
-        // s: sign of (-8 x / top) - (k + 1/2) = sign of (-8 x - (k + 1/2) top) / top
-        const float s = fmaf(-(k + 0.5f), top, -8.0f * x);
-        q = int(k) + (s == 0.0f || ((s > 0.0f) == (top > 0.0f)) ? 1 : 0);
-    }
-    return min(15, max(0, q + 8));
+// floor(t + 1/2) for t = -8 x / top, known to within 1e-5, where it lies near a border b = k +- 1/2 of k = round(t):
+// t - b = (-8 x - b top) / top, and the numerator's sign is that of one fma.
+__device__ __noinline__ float q4_border(float x, float top, float t, float k) {
+    const float b = k + (t > k ? 0.5f : -0.5f), s = fmaf(-b, top, -8.0f * x);
+    return b + (s == 0.0f || ((s > 0.0f) == (top > 0.0f)) ? 0.5f : -0.5f);
 }
 
 __device__ __forceinline__ uint32_t quant8_q4(const float (&x)[8], __half &d) {
@@ -214,7 +187,7 @@ __device__ __forceinline__ uint32_t quant8_q4(const float (&x)[8], __half &d) {
     int key = 1 << 20;
 #pragma unroll
     for (int i = 7; i >= 0; --i)
-        if (fabsf(clamp_kv(x[i])) == M) key = (((threadIdx.x & 3) * 8 + i) << 1) | (x[i] < 0.0f ? 1 : 0);
+        if (fabsf(x[i]) >= M) key = (((threadIdx.x & 3) * 8 + i) << 1) | (x[i] < 0.0f ? 1 : 0);
     key = min(key, __shfl_xor_sync(0xffffffffu, key, 1));
     key = min(key, __shfl_xor_sync(0xffffffffu, key, 2));
     if (mb > 0x7F800000u) {  // after the shuffles, which every lane of the warp takes part in
@@ -227,23 +200,17 @@ __device__ __forceinline__ uint32_t quant8_q4(const float (&x)[8], __half &d) {
         d = __float2half_rn(0.0f);
         return 0x88888888u;
     }
+    // nibble = min(15, floor(t + 8.5)), t = -8 x / top within [-8, 8]; from 7.25 on it is 15
+    const float up = M < 0x1p-100f ? 0x1p100f : 1.0f, ts = top * up;
+    const float inv = __fdividef(-8.0f, ts);
     uint32_t w = 0;  // nibble i = value i
-    if (M >= 0x1p-100f && M < kKvMax) {
-        const float inv = __fdividef(-8.0f, top);
-        float far = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float t = x[i] * inv, m = fminf(t, 7.25f) + (kKvMagic + 8.0f);  // (code 15 is the last)
-            far = fmaxf(far, t > 7.25f ? 0.0f : fabsf(t - (m - (kKvMagic + 8.0f))));
-            w |= (__float_as_uint(m) & 15u) << (4 * i);
-        }
-        if (far < kKvNear) return w;
-        w = 0;
+    for (int i = 0; i < 8; ++i) {
+        const float c = clamp_kv(x[i]) * up, t = fminf(c * inv, 7.25f), m = t + (kKvMagic + 8.0f), k = m - (kKvMagic + 8.0f);
+        uint32_t r = __float_as_uint(m);
+        if (fabsf(t - k) >= kKvNear) r = __float_as_uint(q4_border(c, ts, t, k) + (kKvMagic + 8.0f));
+        w |= (r & 15u) << (4 * i);
     }
-    const float up = M < 0x1p-100f ? 0x1p100f : 1.0f;
-    const float ts = top * up, inv = -8.0f / ts;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w |= uint32_t(q4_code(clamp_kv(x[i]) * up, ts, inv)) << (4 * i);
     return w;
 }
 
@@ -301,16 +268,20 @@ __device__ __forceinline__ void load_row(const uint8_t *data, const __half *scal
         const uint2 w = __ldg(reinterpret_cast<const uint2 *>(data + row * D + l * 8));
         const float d = __half2float(__ldg(scales + row * (D / 32) + (l >> 2)));
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            x[i] = float(int8_t((i < 4 ? w.x : w.y) >> (8 * (i & 3)))) * d;
+        for (int i = 0; i < 8; ++i) {  // code + 128 in the last byte of 2^23
+            const uint32_t b = __byte_perm((i < 4 ? w.x : w.y) ^ 0x80808080u, 0x4B000000u, 0x7650 | (i & 3));
+            x[i] = (__uint_as_float(b) - 8388736.0f) * d;
+        }
     } else {
         const uint2 w =
             __ldg(reinterpret_cast<const uint2 *>(data + row * (D / 2) + (l >> 2) * 16 + (l & 1) * 8));
         const float d = __half2float(__ldg(scales + row * (D / 32) + (l >> 2)));
         const int sh = (l & 2) ? 4 : 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            x[i] = float(int(((i < 4 ? w.x : w.y) >> (8 * (i & 3) + sh)) & 15u) - 8) * d;
+        for (int i = 0; i < 8; ++i) {  // the nibble in the last byte of 2^23
+            const uint32_t n = ((i < 4 ? w.x : w.y) >> (8 * (i & 3) + sh)) & 15u;
+            x[i] = (__uint_as_float(n | 0x4B000000u) - 8388616.0f) * d;
+        }
     }
 }
 
