@@ -23,6 +23,11 @@
 
 namespace anvil {
 
+// How far (in powers of two) a row's reference lies below the largest score when it is chosen, where weights are
+// fp16: those lose bits below 2^-14 and end at 2^-25, so that with 2^6 for the largest, keys of 2^-31 of it still count and
+// a first key with a high score does not drown thousands of low ones.  (bf16 weights have fp32's range.)
+template <bool BF16> constexpr float kAttnHead = BF16 ? 0.0f : 6.0f;
+
 struct AttnIO {
     const void *q;
     int64_t q_row, q_head;  // in values
@@ -288,11 +293,6 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {

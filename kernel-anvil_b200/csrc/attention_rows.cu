@@ -32,7 +32,7 @@ namespace anvil {
 constexpr int kRowsWarps = 4;
 constexpr int kRowsStep = 16;   // keys of a warp's step
 constexpr int kRowsKeys = 64;   // keys of a key tile: one step of each warp
-constexpr float kRowsSlack = 16384.0f;  // the largest weight
+constexpr float kRowsSlack = 60000.0f;  // the largest weight: fp16 ends at 65504
 constexpr int kRowsCost = 0;    // beginning and ending a unit, in key tiles
 
 template <int KIND, int D, int NT> struct RowsShape {
@@ -40,13 +40,13 @@ template <int KIND, int D, int NT> struct RowsShape {
     static constexpr int rb = KvRow<KIND, D>::bytes;
     static constexpr int ch = rb / 16;                      // 16-byte chunks of a row
     static constexpr int sb = KvRow<KIND, D>::scales * 2;   // bytes of a row's scales
-    static constexpr int kst = rb >= 128 ? rb + 16 : rb;    // row strides in the ring
+    static constexpr int kst = KIND == kKvQ8_0 ? rb + 32 : rb + 16;  // row strides in the ring: distinct banks
     static constexpr int vst = rb + 16;
     static constexpr int off_v = kRowsStep * kst, off_s = off_v + kRowsStep * vst;
     static constexpr int off_bad = off_s + 2 * kRowsStep * sb;
     static constexpr int stage = off_bad + 16;
     // two stages keep 16 keys of every warp in flight while 16 are worked on; short rows take more
-    static constexpr int stages = stage <= 1400 ? 4 : stage <= 2800 ? 3 : 2;
+    static constexpr int stages = stage <= 3000 ? 3 : 2;
     static constexpr int ring = stage * stages;             // of one warp
     static constexpr int join = rows * (D + 4) * 4 + rows * 8;  // of one warp, reuses the ring
     static constexpr int per_warp = ((ring > join ? ring : join) + 15) & ~15;
@@ -94,18 +94,13 @@ __device__ __forceinline__ uint32_t q4_fix_high(uint32_t h) { return h2fma(h, 0x
 // ---- the dimension that a lane's operand stands for -------------------------------------------
 
 // First of the 4 dimensions of QK step s for quad lane c; the operands hold (d, d+1), (d+2, d+3), or
-// for Q4_0, whose nibbles come in pairs two bytes apart, (d, d+2), (d+1, d+3).  Chunk j of a lane is
-// 8 (j / 2) + 2 c + j % 2 (rows of 8 chunks and more) or c.
-template <int CH> __device__ __forceinline__ int k_chunk(int j, int c) {
-    return CH >= 8 ? 8 * (j >> 1) + 2 * c + (j & 1) : c;
-}
-template <int KIND, int D> __device__ __forceinline__ int k_dim(int s, int c) {
-    constexpr int CH = KvRow<KIND, D>::bytes / 16;
-    if constexpr (KIND == kKvQ8_0) return 16 * k_chunk<CH>(s >> 2, c) + 4 * (s & 3);
-    else if constexpr (KIND == kKvQ4_0) {
-        if constexpr (D == 64) return 32 * (c >> 1) + 8 * (c & 1) + 4 * (s >> 1) + 16 * (s & 1);
-        else return 32 * k_chunk<CH>(s >> 3, c) + 4 * ((s & 7) >> 1) + 16 * (s & 1);
-    } else return 8 * k_chunk<CH>(s >> 1, c) + 4 * (s & 1);
+// for Q4_0, whose nibbles come in pairs two bytes apart, (d, d+2), (d+1, d+3).  Of a quantised row two steps
+// cover a block of 32 values; 16-bit rows are read in chunks of 8 values, chunk j of a lane 8 (j / 2) + 2 c + j % 2.
+__device__ __forceinline__ int k_chunk(int j, int c) { return 8 * (j >> 1) + 2 * c + (j & 1); }
+template <int KIND> __device__ __forceinline__ int k_dim(int s, int c) {
+    if constexpr (KIND == kKvQ8_0) return 32 * (s >> 1) + 8 * c + 4 * (s & 1);
+    else if constexpr (KIND == kKvQ4_0) return 32 * (s >> 1) + 4 * c + 16 * (s & 1);
+    else return 8 * k_chunk(s >> 1, c) + 4 * (s & 1);
 }
 
 // The i-th (of D / 8) dimension that lane group g (0..7) owns in O^T.
@@ -242,7 +237,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
 #pragma unroll
             for (int s = 0; s < NS; ++s) {
                 uint2 w = make_uint2(0, 0);
-                if (live) w = __ldg(reinterpret_cast<const uint2 *>(src + k_dim<KIND, D>(s, cq)));
+                if (live) w = __ldg(reinterpret_cast<const uint2 *>(src + k_dim<KIND>(s, cq)));
                 qb[t][s][0] = w.x;
                 qb[t][s][1] = w.y;
                 if (S::quant) {
@@ -323,53 +318,67 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) sc2[t][j] = 0.0f;
-            auto mul = [&](int s2, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-                const uint32_t a[4] = {a0, a1, a2, a3};
-#pragma unroll
-                for (int t = 0; t < NT; ++t) mma16816<BF>(sc2[t], a, qb[t][s2][0], qb[t][s2][1]);
-            };
-            auto scale_of = [&](int row, int dim) { return dup16(__half_as_ushort(ks[row * (D / 32) + dim / 32])); };
-            auto q4_steps = [&](int s2, uint32_t u, uint32_t v, uint32_t d, uint32_t e) {  // words of keys g, g + 8
-                const uint32_t u8 = u >> 8, v8 = v >> 8;
-                mul(s2, h2mul(q4_fix_low(q4_low(u)), d), h2mul(q4_fix_low(q4_low(v)), e), h2mul(q4_fix_low(q4_low(u8)), d),
-                    h2mul(q4_fix_low(q4_low(v8)), e));
-                mul(s2 + 1, h2mul(q4_fix_high(q4_high(u)), d), h2mul(q4_fix_high(q4_high(v)), e),
-                    h2mul(q4_fix_high(q4_high(u8)), d), h2mul(q4_fix_high(q4_high(v8)), e));
-            };
             const uint8_t *k0 = sk + g * S::kst, *k1 = k0 + 8 * S::kst;
-            if constexpr (KIND == kKvQ4_0 && D == 64) {
-                const uint2 u = *reinterpret_cast<const uint2 *>(k0 + cq * 8), v = *reinterpret_cast<const uint2 *>(k1 + cq * 8);
-                const uint32_t d = scale_of(g, k_dim<KIND, D>(0, cq)), e = scale_of(g + 8, k_dim<KIND, D>(0, cq));
-                q4_steps(0, u.x, v.x, d, e);
-                q4_steps(2, u.y, v.y, d, e);
+            if constexpr (S::quant) {
+                // Codes are whole numbers of fp16, taken exactly; a block's sum is multiplied by its scale in fp32.  (The
+                // scale times the codes, rounded to fp16, was the largest error of the scores, and more instructions.)
+                constexpr int NB = D / 32;
+                uint32_t dw[2][NB / 2];  // scales of keys g and g + 8
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const __half *at = ks + (g + 8 * i) * NB;
+                    if constexpr (NB == 2) dw[i][0] = *reinterpret_cast<const uint32_t *>(at);
+                    else
+#pragma unroll
+                        for (int j = 0; j < NB / 4; ++j)
+                            *reinterpret_cast<uint2 *>(&dw[i][2 * j]) = *reinterpret_cast<const uint2 *>(at + 4 * j);
+                }
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    float x[NT][4] = {};
+                    uint32_t lo[4], hi[4];  // the block's two steps
+                    if constexpr (KIND == kKvQ8_0) {
+                        uint2 u = *reinterpret_cast<const uint2 *>(k0 + b * 32 + cq * 8), v = *reinterpret_cast<const uint2 *>(k1 + b * 32 + cq * 8);
+                        u.x ^= 0x80808080u, u.y ^= 0x80808080u, v.x ^= 0x80808080u, v.y ^= 0x80808080u;
+                        lo[0] = q8_pair(u.x, 0x4140), lo[1] = q8_pair(v.x, 0x4140), lo[2] = q8_pair(u.x, 0x4342), lo[3] = q8_pair(v.x, 0x4342);
+                        hi[0] = q8_pair(u.y, 0x4140), hi[1] = q8_pair(v.y, 0x4140), hi[2] = q8_pair(u.y, 0x4342), hi[3] = q8_pair(v.y, 0x4342);
+                    } else {
+                        const uint32_t u = *reinterpret_cast<const uint32_t *>(k0 + b * 16 + cq * 4), v = *reinterpret_cast<const uint32_t *>(k1 + b * 16 + cq * 4);
+                        const uint32_t u8 = u >> 8, v8 = v >> 8;
+                        lo[0] = q4_fix_low(q4_low(u)), lo[1] = q4_fix_low(q4_low(v)), lo[2] = q4_fix_low(q4_low(u8)), lo[3] = q4_fix_low(q4_low(v8));
+                        hi[0] = q4_fix_high(q4_high(u)), hi[1] = q4_fix_high(q4_high(v)), hi[2] = q4_fix_high(q4_high(u8)), hi[3] = q4_fix_high(q4_high(v8));
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        mma16816<BF>(x[t], lo, qb[t][2 * b][0], qb[t][2 * b][1]);
+                        mma16816<BF>(x[t], hi, qb[t][2 * b + 1][0], qb[t][2 * b + 1][1]);
+                    }
+                    float d[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float y = __half2float(__ushort_as_half(uint16_t(dw[i][b >> 1] >> (16 * (b & 1)))));
+                        d[i] = fmaf(0.0f, y, y);  // an infinite scale is NaN, as zero codes times it are
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) sc2[t][j] = fmaf(x[t][j], d[j >> 1], sc2[t][j]);
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < S::ch / 4; ++j) {
-                    const int at = k_chunk<S::ch>(j, cq) * 16;
-                    const uint4 u4 = *reinterpret_cast<const uint4 *>(k0 + at), v4 = *reinterpret_cast<const uint4 *>(k1 + at);
-                    const uint32_t u[4] = {u4.x, u4.y, u4.z, u4.w}, v[4] = {v4.x, v4.y, v4.z, v4.w};
-                    if constexpr (KIND == kKvQ8_0) {
-                        const int dim = k_dim<KIND, D>(4 * j, cq);
-                        const uint32_t d = scale_of(g, dim), e = scale_of(g + 8, dim);
+                    const int at = k_chunk(j, cq) * 16;
+                    const uint4 u = *reinterpret_cast<const uint4 *>(k0 + at), v = *reinterpret_cast<const uint4 *>(k1 + at);
+                    const uint32_t a0[4] = {u.x, v.x, u.y, v.y}, a1[4] = {u.z, v.z, u.w, v.w};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint32_t x = u[i] ^ 0x80808080u, y = v[i] ^ 0x80808080u;
-                            mul(4 * j + i, h2mul(q8_pair(x, 0x4140), d), h2mul(q8_pair(y, 0x4140), e),
-                                h2mul(q8_pair(x, 0x4342), d), h2mul(q8_pair(y, 0x4342), e));
-                        }
-                    } else if constexpr (KIND == kKvQ4_0) {
-                        const int dim = k_dim<KIND, D>(8 * j, cq);
-                        const uint32_t d = scale_of(g, dim), e = scale_of(g + 8, dim);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) q4_steps(8 * j + 2 * i, u[i], v[i], d, e);
-                    } else {
-                        mul(2 * j, u[0], v[0], u[1], v[1]);
-                        mul(2 * j + 1, u[2], v[2], u[3], v[3]);
+                    for (int t = 0; t < NT; ++t) {
+                        mma16816<BF>(sc2[t], a0, qb[t][2 * j][0], qb[t][2 * j][1]);
+                        mma16816<BF>(sc2[t], a1, qb[t][2 * j + 1][0], qb[t][2 * j + 1][1]);
                     }
                 }
             }
 
-            // ---- weights by the rows' references m.  Only where one exceeds 2^14 (fp16 ends at 65504), or where there is
+            // ---- weights by the rows' references m.  Only where one exceeds 60000, or where there is
             // no reference yet, is the step's maximum looked for, made the reference, and the step taken again.
             const int key0 = s * kRowsStep;
             const bool masked = key0 + kRowsStep > free_end || bad != 0;
@@ -402,7 +411,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                         float x = fmaxf(sc2[t][d], sc2[t][2 + d]);
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * fac[t][d];
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16)) * fac[t][d] - kAttnHead<BF>;
                         const float mn = fmaxf(m[t][d], x);
                         const float a = mn == -INFINITY ? 1.0f : ex2(m[t][d] - mn);
                         fresh |= mn == -INFINITY;  // a row without keys so far

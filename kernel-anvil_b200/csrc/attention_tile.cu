@@ -34,7 +34,7 @@ constexpr int kTileThreads = 512;   // 128 registers a thread at launch, divided
 constexpr int kTileLoaders = 128;   // threads of the four loading warps
 constexpr int kTileCost = 8;        // beginning and ending a unit, in key tiles
 constexpr int kTileBulkShift = 4;   // pages of 16 keys: their scales are whole 16-byte pieces
-constexpr float kTileSlack = 32768.0f;  // the largest sum of a tile's weights, and so weight
+constexpr float kTileSlack = 60000.0f;  // the largest sum of a tile's weights, and so weight: fp16 ends at 65504
 
 template <int KIND, int D> struct TileShape {
     static constexpr int nq = D == 256 ? 1 : 2;         // row tiles of 128
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
                                 for (int i = 0; i < 64; i += 2)
                                     mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac;
+                                const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fac - kAttnHead<BF>;
                                 const float mn = raise && mt > m ? mt : m;
                                 const float a = mn > m ? ex2(m - mn) : 1.0f;
                                 if (t > u.t0) {
@@ -962,6 +962,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         __syncwarp();
     }
     fence_before();
+    __syncthreads();
+    // a wait gave up: what is still on its way to shared memory gets a millisecond to land
+    if (*reinterpret_cast<volatile int *>(&sh.failed))
+        for (const uint64_t t = global_timer_ns(); global_timer_ns() - t < 1000000;) __nanosleep(1000);
     __syncthreads();
     if (warp == 12) {
         fence_after();

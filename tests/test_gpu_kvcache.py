@@ -507,3 +507,54 @@ def test_refusals_on_the_gpu():
     with pytest.raises(AnvilError):
         ops.kv_read(cache, table, start, 2, out=(k[:1], k))
     assert mmvq.take_device_status() == 0
+
+
+# ---- the corners of the two kernels' loads and divisions ---------------------------------------
+
+@pytest.mark.parametrize("kind,dtype", [("F16", "f16"), ("BF16", "bf16"), ("Q8_0", "f16"), ("Q4_0", "bf16")])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 2, 4, 8])
+@pytest.mark.parametrize("q_lens", [[1, 3], [2, 45]])
+def test_attention_pages_smaller_than_a_load(kind, dtype, dim, page, q_lens):
+    batch = ref.Batch(kind, dim, 2, page, q_lens, [77, 130], seed=page, wide=1)
+    batch.poison()
+    check_attention(batch, 4, dtype)
+
+
+@pytest.mark.parametrize("q_step,kind,dtype", [(2, "Q4_0", "f16"), (17, "F16", "f16"), (17, "Q8_0", "bf16")])
+def test_attention_more_sequences_than_threads(q_step, kind, dtype):
+    """The place of a share is found in several passes over the batch."""
+    lens = [(37 * i) % 90 for i in range(1100)]
+    batch = ref.Batch(kind, 64, 1, 16, [(i * 7) % q_step if n else 0 for i, n in enumerate(lens)], lens, seed=12)
+    check_attention(batch, 4, dtype)
+
+
+@pytest.mark.parametrize("kind,dtype", [("F16", "f16"), ("Q8_0", "f16"), ("BF16", "bf16")])
+@pytest.mark.parametrize("q_len", [1, 12])
+def test_one_high_score_does_not_drown_thousands_of_low_ones(kind, dtype, q_len):
+    """The first key's score is 17 above all others', which are equal, and only the others have values.
+
+    Scores are exact.  A weight is rounded by u_p of itself and, in fp16, by 2^-31 of the largest weight at least;
+    exponentials and sums take 2^-18 (16 (n + D) 2^-24), and the output is rounded once.
+    """
+    n, batch_size, kv_heads, dim = 2000, 48, 8, 64
+    batch = ref.Batch(kind, dim, kv_heads, 16, [q_len], [n], seed=13)
+    x = torch.zeros(batch.k.shape[0], kv_heads, 16, dim)
+    batch.v, batch.vs = ref.quantise(kind, torch.ones_like(x))
+    p, o = batch.slots(0, 0)
+    x[p, :, o, 0] = 17.0
+    batch.k, batch.ks = ref.quantise(kind, x)
+    key, one = batch.rows_of("k", 0)[0, 0, 0], batch.rows_of("v", 0)[1, 0, 0]
+    batch.set_token("v", 0, 0, 0.0)
+    q = torch.zeros(batch_size * q_len, 4 * kv_heads, dim, dtype=ref.NP[dtype], device="cuda")
+    q[..., 0] = 1.0
+    got = ops.paged_attention(q, batch.cache(ops), batch.table.cuda().expand(batch_size, -1).contiguous(),
+                              torch.arange(batch_size + 1, dtype=torch.int32, device="cuda") * q_len,
+                              torch.full((batch_size,), n, dtype=torch.int32, device="cuda"), scale=1.0)
+    seen = (n - q_len + 1 + torch.arange(q_len).double()).repeat(batch_size)[:, None, None]
+    w = (seen - 1) * torch.exp(-key)
+    want = one * w / (1 + w)
+    u = ref.U[ref.NP[dtype]]
+    tol = want * (2 * u + (2.0 ** -11 if batch.ks is not None else 0) + 2.0 ** -18 + 16 * (n + dim) * 2.0 ** -24)
+    error = (got.cpu().double() - want).abs()
+    assert (error <= tol + seen * 2.0 ** -31 + 2.0 ** -25).all(), (error / want).max()
