@@ -43,7 +43,8 @@ static AttnPlan attn_plan(const anvil_kv_cache *c, const KvCacheView &cv, const 
     const int group = heads / cv.kv_heads;
     AttnPlan p;
     const int64_t rows = int64_t(bv.total) * group;
-    p.nt = rows <= int64_t(bv.batch) * 8 ? 1 : rows <= int64_t(bv.batch) * 16 ? 2 : 0;
+    const int64_t few = int64_t(bv.batch) * (c->kind == kKvQ8_0 || (c->kind == kKvQ4_0 && c->head_dim < 256) ? 32 : 16);
+    p.nt = rows <= int64_t(bv.batch) * 8 ? 1 : rows <= few ? 2 : 0;
     const AttnTiles t = p.nt ? attn_rows_tiles(c->kind, c->head_dim, p.nt) : attn_tile_tiles(c->head_dim);
     const int64_t capacity = std::min<int64_t>(int64_t(bv.max_pages) << cv.page_shift, 0x7fffffff);
     const int64_t units = int64_t(cv.kv_heads) * (int64_t(bv.total) * group / t.rows + std::min(bv.batch, bv.total));

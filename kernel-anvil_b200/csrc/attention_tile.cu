@@ -51,8 +51,12 @@ template <int KIND, int D> struct TileShape {
     static constexpr int jobs = D == 256 ? 2 : 1;
     // quantised: a job's codes and scales as they are in the cache
     static constexpr int rb = KvRow<KIND, D>::bytes, sb = KvRow<KIND, D>::scales * 2;
-    static constexpr int raw = quant ? keys * (rb + sb) * 2 / jobs : 0;
-    static constexpr int nraw = D == 256 && KIND == kKvQ8_0 ? 1 : 3;
+    // (of Q8_0 with head_dim 256 half a job: one whole job has room beside the operands, and waiting for every job's
+    // copies took twice the time)
+    static constexpr int halves = D == 256 && KIND == kKvQ8_0 ? 2 : 1;
+    static constexpr int raw_keys = keys / halves;
+    static constexpr int raw = quant ? raw_keys * (rb + sb) * 2 / jobs : 0;
+    static constexpr int nraw = 3;
     static constexpr int smem = 1024 + q_bytes + 2 * nbuf * buf + nraw * raw;
     // tensor memory columns: two turns of S for each row tile, then O
     static constexpr int s_cols = keys, o_col = 4 * keys, o_cols = D;
@@ -711,7 +715,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             };
             constexpr uint32_t flip = KIND == kKvQ8_0 ? 0x80808080u : 0;
             // a job's codes from the raw buffer that warp 14 had filled
-            auto from_raw = [&](const TileUnit<KIND, D> &u, int t) {
+            auto from_raw = [&](const TileUnit<KIND, D> &u, int t, int half) {
                 const int slot = taken % S::nraw;
                 tile_wait(&sh, &sh.raw_full[slot], (taken / S::nraw) & 1, limit_ns);
                 __syncwarp();
@@ -720,9 +724,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 const uint32_t bad[2] = {sh.bad[seq & 7][0], sh.bad[seq & 7][1]};
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-                    const int r = r0 + i % R * STEP, v = i / R;
-                    const uint4 x = *reinterpret_cast<const uint4 *>(raw + (v * S::keys + r) * RB + ch * 16);
-                    const uint32_t y = *reinterpret_cast<const uint16_t *>(raw + N / R * S::keys * RB + (v * S::keys + r) * S::sb + ch * VALS / 32 * 2);
+                    if (i * S::halves / N != half) continue;
+                    const int r = r0 + i % R * STEP, v = i / R, at = v * S::raw_keys + r - half * S::raw_keys;
+                    const uint4 x = *reinterpret_cast<const uint4 *>(raw + at * RB + ch * 16);
+                    const uint32_t y = *reinterpret_cast<const uint16_t *>(raw + N / R * S::raw_keys * RB + at * S::sb + ch * VALS / 32 * 2);
                     w[i] = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
                     d[i] = r >= left || ((bad[r >> 5] >> (r & 31)) & 1) ? 0 : dup16(y);
                 }
@@ -796,10 +801,22 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                 load_q(u);
                 if (bulk) {
                     for (int t = u.t0; t < u.t1; ++t, ++seq)
-                        for (int job = 0; job < jobs; ++job, ++taken) {
-                            from_raw(u, t);
+                        for (int job = 0; job < jobs; ++job) {
+                            // (Raw buffers are given back when their codes are in registers where they hold half a job, else
+                            // after the widening, which took 4% less.)
+#pragma unroll
+                            for (int half = 0; half < S::halves; ++half) {
+                                from_raw(u, t, half);
+                                if (S::halves == 1) break;
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(&sh.raw_empty[taken % S::nraw]);
+                                ++taken;
+                            }
                             widen(job, job == jobs - 1 && (t + 1) * S::keys > u.free_end);
-                            if (lane == 0) mbar_arrive(&sh.raw_empty[taken % S::nraw]);
+                            if (S::halves == 1) {
+                                if (lane == 0) mbar_arrive(&sh.raw_empty[taken % S::nraw]);
+                                ++taken;
+                            }
                         }
                 } else {
                     // pages of a few keys: every thread fetches its own, a job ahead of the widening
@@ -905,7 +922,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         if (warp == 14 && S::quant && c.page_shift >= kTileBulkShift) {
             // ================= raw buffers: bulk copies, page by page ====================================
-            const int per = min(S::keys, 1 << c.page_shift), parts = S::keys / per;  // keys of a copy, copies of a tile
+            const int per = min(S::raw_keys, 1 << c.page_shift), parts = S::keys / per;  // keys of a copy, copies of a tile
             uint32_t filled = 0;
             int seq = 0;
             while (p.b < bt.batch && p.unit0 < hi) {
@@ -921,12 +938,13 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                     const int64_t row = here ? kv_row(page, c.num_pages, p.head, c.kv_heads, key & ((1 << c.page_shift) - 1), c.page_shift) : -1;
                     page = page_of(t + 1);
                     const uint32_t live = __ballot_sync(0xffffffffu, row >= 0), none = __ballot_sync(0xffffffffu, here && row < 0);
-                    for (int job = 0; job < S::jobs; ++job, ++filled) {
+                    for (int piece = 0; piece < S::jobs * S::halves; ++piece, ++filled) {
+                        const int job = piece / S::halves, half = piece % S::halves, i0 = half * (parts / S::halves), i1 = i0 + parts / S::halves;
                         const int slot = filled % S::nraw;
                         if (filled >= S::nraw) tile_wait(&sh, &sh.raw_empty[slot], (filled / S::nraw - 1) & 1, limit_ns);
                         __syncwarp();
                         if (lane == 0) {
-                            if (job == 0) {
+                            if (piece == 0) {
                                 uint64_t bad = 0;
                                 for (int i = 0; i < parts; ++i)
                                     if ((none >> i) & 1) bad |= (per == 64 ? ~uint64_t(0) : (uint64_t(1) << per) - 1) << (i * per);
@@ -934,19 +952,19 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                                 sh.bad[seq & 7][1] = uint32_t(bad >> 32);
                                 if (bad) flag_bad_page();
                             }
-                            mbar_arrive_expect_tx(&sh.raw_full[slot], __popc(live) * per * (S::rb + S::sb) * 2 / S::jobs);
+                            mbar_arrive_expect_tx(&sh.raw_full[slot], __popc(live >> i0 << (32 - i1 + i0)) * per * (S::rb + S::sb) * 2 / S::jobs);
                         }
                         __syncwarp();
                         uint8_t *raw = sraw + slot * S::raw;
-                        for (int i = 0; i < parts; ++i) {
+                        for (int i = i0; i < i1; ++i) {
                             const int64_t first = __shfl_sync(0xffffffffu, row, i);
                             if (first >= 0 && elect_one()) {
 #pragma unroll
                                 for (int v = 0; v < 2 / S::jobs; ++v) {
                                     const bool values = S::jobs == 2 ? job == 1 : v == 1;
-                                    bulk_copy_g2s(raw + (v * S::keys + i * per) * S::rb, (values ? c.v : c.k) + first * S::rb,
+                                    bulk_copy_g2s(raw + (v * S::raw_keys + (i - i0) * per) * S::rb, (values ? c.v : c.k) + first * S::rb,
                                                   per * S::rb, &sh.raw_full[slot]);
-                                    bulk_copy_g2s(raw + 2 / S::jobs * S::keys * S::rb + (v * S::keys + i * per) * S::sb,
+                                    bulk_copy_g2s(raw + 2 / S::jobs * S::raw_keys * S::rb + (v * S::raw_keys + (i - i0) * per) * S::sb,
                                                   reinterpret_cast<const uint8_t *>(values ? c.vs : c.ks) + first * S::sb, per * S::sb,
                                                   &sh.raw_full[slot]);
                                 }
