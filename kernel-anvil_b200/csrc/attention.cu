@@ -43,6 +43,15 @@ static AttnPlan attn_plan(const anvil_kv_cache *c, const KvCacheView &cv, const 
     const int group = heads / cv.kv_heads;
     AttnPlan p;
     const int64_t rows = int64_t(bv.total) * group;
+    // Few rows a sequence go to the rows kernel, in tiles of 8 or 16; the tile kernel, whose tiles have 128 rows,
+    // takes the others.  Where they cross, 16 sequences of 6000 keys in 8 heads of 128, us by rows a sequence and head:
+    //                 8: 8 / 16 / tile     16: 8 / 16 / tile     32: 16 / tile     48: 16 / tile
+    //   F16              83 /  84 /  95      141 /  87 /  94       149 /  97         216 /  98
+    //   Q8_0             52 /  60 / 113       86 /  63 / 113       106 / 115         152 / 117
+    //   Q4_0             52 /  63 / 152       87 /  66 / 152       111 / 154         159 / 156
+    // (a second tile of rows reads a 16-bit cache, which is what bounds it, once more, and widens quantised codes once
+    // more, which the tile kernel does more slowly: through shared memory).  head_dim 256 and 4000 keys, 32 rows: Q8_0 133 /
+    // 253, Q4_0 170 / 144.  Averages over the batch: the lengths are on the device.
     const int64_t few = int64_t(bv.batch) * (c->kind == kKvQ8_0 || (c->kind == kKvQ4_0 && c->head_dim < 256) ? 32 : 16);
     p.nt = rows <= int64_t(bv.batch) * 8 ? 1 : rows <= few ? 2 : 0;
     const AttnTiles t = p.nt ? attn_rows_tiles(c->kind, c->head_dim, p.nt) : attn_tile_tiles(c->head_dim);

@@ -9,7 +9,7 @@
 // S has two turns of 64 columns a row tile, so the scores of the next keys are there when the weights of
 // the last ones are done, and the softmax never waits for a product that waits for it.  (Tiles of 128
 // keys fill tensor memory with one turn, P over S: the chain softmax, P V, Q K^T, softmax then left
-// both sides idle half of the time: 2.68 against FILLCHUNK ms for 2048 rows over 30049 keys.)
+// both sides idle half of the time: 2.68 against 2.19 ms for 2048 rows of 64 heads over 30049 keys of Q8_0.)
 // Warp roles: warps 0-3 and 4-7 are the softmax of the two row tiles; warps 8-11 bring keys and values
 // through the page table into a ring of buffers in the 128-byte swizzled layout, widening quantised
 // codes to fp16 on the way, and a unit's queries while the softmax is at the unit before; warps 12 and 13
@@ -17,9 +17,15 @@
 // hand over, more than the products took); warp 14 fetches quantised codes.  All hand-over is by mbarriers;
 // each wait is bounded and a failure makes the later ones return at once.
 //
-// Weights are taken by a reference, the maximum of a row's first tile; it is raised, and O rescaled, only when
-// a tile's weights sum to more than 2^15 (fp16 and fp32 hold them without loss), which the sum that
-// is taken anyway shows: most tiles are never searched for their maximum.
+// Weights are taken by a reference, which a row's first tile sets near its maximum; it is raised, and O rescaled,
+// only when a tile's weights sum to more than fp16 holds, which the sum that is taken anyway shows: most tiles are
+// never searched for their maximum.  P is rounded to the products' 16-bit type (fp16 2^-11, bf16 2^-8 of each weight) and
+// quantised keys and values to fp16 (2^-11), since the products take 16 bits; scores, sums and outputs are fp32.
+//
+// What bounds it: the softmax, some 2000 cycles for the 64 keys of 256 rows (64 exponentials, as many roundings and the moves
+// from and to tensor memory a thread, four warps a scheduler); the products take about 1300.  7993 rows of 64 heads of 128 over themselves, BF16,
+// take 0.55 ms, 950 TFLOP/s or 57% of the measured GEMM rate; 2048 over 30049 keys of Q8_0 2.19 ms, 890 TFLOP/s.
+// Short sequences pay kTileCost for each unit: 12 sequences of 1 to 600 new tokens 0.36 ms, 490 TFLOP/s.
 #include <cuda.h>
 
 #include <algorithm>
@@ -32,8 +38,13 @@ namespace anvil {
 
 constexpr int kTileThreads = 512;   // 128 registers a thread at launch, divided anew by warp group below
 constexpr int kTileLoaders = 128;   // threads of the four loading warps
-constexpr int kTileCost = 8;        // beginning and ending a unit, in key tiles
-constexpr int kTileBulkShift = 4;   // pages of 16 keys: their scales are whole 16-byte pieces
+// Beginning and ending a unit, in key tiles.  Counted as 2 / 4 / 8 / 12: 644 / 592 / 564 / 577 us for a prompt of 7993
+// tokens, 463 / 389 / 393 / 435 for 12 sequences of 1 to 600 new ones.
+constexpr int kTileCost = 8;
+// Quantised pages of 16 keys and more, whose scales are whole 16-byte pieces, come by bulk copies: 1000 rows of 32 heads over
+// 16000 keys in pages of 16 take 326 us (Q8_0) and 357 (Q4_0), by plain loads 440 and 383.  (16-bit pages of 8 keys
+// and more by TMA: 382 us at 8 and 283 at 16 keys a page, by cp.async 551.)
+constexpr int kTileBulkShift = 4;
 constexpr float kTileSlack = 60000.0f;  // the largest sum of a tile's weights, and so weight: fp16 ends at 65504
 
 template <int KIND, int D> struct TileShape {
@@ -315,9 +326,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                             for (int i = 0; i < 64; ++i)
                                 if (i >= left || ((bad[i >> 5] >> (i & 31)) & 1)) s[i] = 0xFF800000u;
                         }
-                        // The weights of this tile by the row's reference m so far; only where their sum shows one beyond
-                        // 2^15 (fp16 ends at 65504), or where there is no reference yet, is the maximum looked for, made
-                        // the reference, and the tile taken again.
+                        // The weights of this tile by the row's reference m so far; only where their sum shows that one may
+                        // be too large, or where there is no reference yet, is the maximum looked for, the reference set by
+                        // it, and the tile taken again.
                         float sum = 0.0f;
                         uint32_t y[32];
                         bool raise = m == -INFINITY;
@@ -695,8 +706,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         } else {
             // 16 bytes of codes a turn: 16 (Q8_0) or 32 (Q4_0) values, two or four chunks; a thread has one chunk of R
             // keys, 128 / CH apart.  Pages of 16 keys and more come through raw buffers that warp 14 fills by bulk copies:
-            // beside 200 KB of shared memory L1 is too small to have many plain loads on their way (they took 1.5 us a
-            // tile, more than the softmax).
+            // beside 200 KB of shared memory L1 is too small to have many plain loads on their way.
             constexpr int RB = S::rb, CH = RB / 16, R = S::keys * CH / LT, STEP = LT / CH;
             constexpr int jobs = S::jobs, N = 2 * R / jobs;
             constexpr int OUT = KIND == kKvQ8_0 ? 2 : 4, VALS = 8 * OUT;
