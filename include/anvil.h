@@ -397,7 +397,7 @@ typedef struct anvil_kv_cache {
  * call's k, v, q and out (start: batch + 1 values, ascending); rows behind start[batch] (of
  * `total`) are neither read nor written.  kv_len[b] tokens of it are in the cache, the new ones
  * included: its row i is at position kv_len[b] - (start[b+1] - start[b]) + i.  Position p is in
- * page page_table[b * page_table_stride + p / page_size].  Entries are read on the device: one
+ * page page_table[b * page_table_stride + p / page_size], p below 2^31 - 4096.  Entries are read on the device: one
  * that is out of range is cut or skipped, never followed, and raises ANVIL_DEVICE_BAD_PAGE. */
 typedef struct anvil_kv_batch {
     const int32_t *page_table;

@@ -55,7 +55,7 @@ static AttnPlan attn_plan(const anvil_kv_cache *c, const KvCacheView &cv, const 
     const int64_t few = int64_t(bv.batch) * (c->kind == kKvQ8_0 || (c->kind == kKvQ4_0 && c->head_dim < 256) ? 32 : 16);
     p.nt = rows <= int64_t(bv.batch) * 8 ? 1 : rows <= few ? 2 : 0;
     const AttnTiles t = p.nt ? attn_rows_tiles(c->kind, c->head_dim, p.nt) : attn_tile_tiles(c->head_dim);
-    const int64_t capacity = std::min<int64_t>(int64_t(bv.max_pages) << cv.page_shift, 0x7fffffff);
+    const int64_t capacity = kv_capacity(bv, cv);
     const int64_t units = int64_t(cv.kv_heads) * (int64_t(bv.total) * group / t.rows + std::min(bv.batch, bv.total));
     const int64_t per = std::max<int64_t>(1, (capacity + t.keys - 1) / t.keys);
     const int64_t slots = 148 * t.occ;

@@ -49,9 +49,13 @@ struct KvBatchView {
     int batch, total;
 };
 
-__device__ __forceinline__ int64_t kv_capacity(const KvBatchView &bt, const KvCacheView &c) {
+// Tokens of a sequence at most: positions of the tiles behind the last one are still ints.
+constexpr int64_t kKvMaxTokens = 0x7ffff000;
+
+// Tokens that a sequence's row of the page table can name.
+__host__ __device__ __forceinline__ int64_t kv_capacity(const KvBatchView &bt, const KvCacheView &c) {
     const int64_t n = int64_t(bt.max_pages) << c.page_shift;
-    return n > 0x7fffffff ? 0x7fffffff : n;
+    return n > kKvMaxTokens ? kKvMaxTokens : n;
 }
 
 __device__ __forceinline__ KvSeq load_seq(const KvBatchView &bt, const KvCacheView &c, int b) {

@@ -558,3 +558,89 @@ def test_one_high_score_does_not_drown_thousands_of_low_ones(kind, dtype, q_len)
     tol = want * (2 * u + (2.0 ** -11 if batch.ks is not None else 0) + 2.0 ** -18 + 16 * (n + dim) * 2.0 ** -24)
     error = (got.cpu().double() - want).abs()
     assert (error <= tol + seen * 2.0 ** -31 + 2.0 ** -25).all(), (error / want).max()
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_the_longest_sequence(q_len):
+    """2^31 - 4096 tokens, one page named over and over: the attention over that page.
+
+    fp32 sums of some 2^31 / 592 / 4 terms a warp, each addition off by 2^-23 of the sum at most: 2^20 2^-23 would be the
+    worst of all, reached only if every addition were cut the same way; a step's 16 to 64 keys are one addition, so
+    2^16 2^-23 = 2^-7, beside the roundings of weights, values and output (3 of 2^-11).
+    """
+    batch = ref.Batch("Q4_0", 64, 1, 1024, [q_len], [1024], seed=14, spare=0)
+    cache, q = batch.cache(ops), make_q(batch, 1, "f16")
+    table, start, kv_len = batch.on_gpu()
+    want = ops.paged_attention(q, cache, table, start, kv_len, causal=False).float()
+    longest = 2 ** 31 - 4096
+    many = torch.zeros(1, 2 ** 21, dtype=torch.int32, device="cuda")
+    bar = (2.0 ** -7 + 4 * 2.0 ** -11) * batch.rows_of("v", 0).abs().max()
+    for n, status in ((longest, 0), (2 ** 31 - 1, ops.BAD_PAGE)):
+        got = ops.paged_attention(q, cache, many, start, torch.tensor([n], dtype=torch.int32).cuda(), causal=False)
+        assert (got.float() - want).abs().max() <= bar
+        assert mmvq.take_device_status() == status
+
+
+@pytest.mark.parametrize("kind,dtype", [("Q8_0", "bf16"), ("F16", "f16")])
+@pytest.mark.parametrize("q_lens", [[1, 3], [40, 70]])
+def test_pages_beyond_the_fourth_gigabyte(kind, dtype, q_lens):
+    batch = ref.Batch(kind, 128, 8, 64, q_lens, [500, 200], seed=15, spare=0)
+    pages = batch.k.shape[0]
+    small = batch.cache(ops)
+    big = ops.PagedKVCache(70000, 64, 8, 128, kind)
+    assert big.k.numel() * big.k.element_size() > 2 ** 32 + 2 ** 28
+    table, start, kv_len = batch.on_gpu()
+    far = torch.where(table < 0, table, table + (70000 - pages))
+    new = torch.randn(2, batch.rows, 8, 128, generator=batch.gen).to(ref.NP[dtype]).cuda()
+    for name in ("k", "v", "k_scale", "v_scale"):
+        if getattr(small, name) is not None:
+            getattr(big, name)[70000 - pages:].copy_(getattr(small, name))
+    q = make_q(batch, 16, dtype)
+    rows = torch.tensor([0, 500, 700], dtype=torch.int32).cuda()
+    got = []
+    for cache, t in ((small, table), (big, far)):
+        ops.kv_write(cache, new[0], new[1], t, start, kv_len)
+        got.append((ops.paged_attention(q, cache, t, start, kv_len), *ops.kv_read(cache, t, rows, 700)))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    assert mmvq.take_device_status() == 0
+
+
+@pytest.mark.parametrize("q_len", [1, 60])
+def test_a_table_without_pages(q_len):
+    batch = ref.Batch("Q8_0", 128, 1, 16, [q_len, 2], [0, 0], spare=1)
+    cache, q = batch.cache(ops), make_q(batch, 4, "bf16")
+    table, start, kv_len = batch.on_gpu()
+    assert table.shape == (2, 0)
+    assert (ops.paged_attention(q, cache, table, start, kv_len) == 0).all()
+    assert mmvq.take_device_status() == 0
+    assert (ops.paged_attention(q, cache, table, start, kv_len + 5) == 0).all()
+    assert mmvq.take_device_status() == ops.BAD_PAGE
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """Kernels are loaded and their attributes set while a stream captures."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from kernel_anvil import kvcache as ops
+table = torch.arange(40, dtype=torch.int32, device="cuda")[None]
+for rows in (1, 100):
+    q = torch.randn(rows, 8, 128, dtype=torch.float16, device="cuda")
+    k = torch.randn(rows, 2, 128, dtype=torch.float16, device="cuda")
+    start = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([600], dtype=torch.int32, device="cuda")
+    cache = ops.PagedKVCache(40, 16, 2, 128, "Q8_0")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.kv_write(cache, k, k, table, start, lens)
+        out = ops.paged_attention(q, cache, table, start, lens)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, ops.paged_attention(q, cache, table, start, lens)) and bool(out.any())
+"""
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(p for p in sys.path if p))
+    subprocess.run([sys.executable, "-c", code], check=True, env=env, timeout=240)
