@@ -14,7 +14,8 @@
 // Both kernels move each byte once.  7993 bf16 tokens of 8 heads of 128: F16 written in 8 us (the L2 takes them), read in 8;
 // Q8_0 18 and 9, Q4_0 24 and 11: the write of the quantised kinds is bound by the instructions that find the
 // codes.  Reading 32801 tokens of Q8_0 as bf16 (206 MB) takes 40 us, 78% of the measured HBM rate, and a decode
-// step's 48 rows 3 us each way, which is the launch.  One lane handles 8 values of a row (16 bytes of a 16-bit input), so a
+// step's 48 rows 3 us each way, which is the launch.  (Two, three or four rows a thread in the read, for more loads on
+// their way, took 43 to 44 us, and a decode step 1 to 2 us more.)  One lane handles 8 values of a row (16 bytes of a 16-bit input), so a
 // block is four neighbouring lanes and its maximum is two shuffles; keys and values of a row are
 // handled by the same lanes, which keeps two independent streams of loads in flight.
 #include <cuda_runtime.h>

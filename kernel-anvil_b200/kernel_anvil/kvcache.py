@@ -259,7 +259,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
         raise _bad(f"a {cache.kind} cache takes q of its own type, got {q.dtype}")
     b = _batch(cache, page_table, q_start, kv_len, q.shape[0])
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=cache.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != cache.device or \
             not out.is_contiguous() or out.data_ptr() % 16:
         raise _bad("out is a contiguous 16-byte aligned tensor of q's shape and type on the cache's device")

@@ -644,3 +644,28 @@ for rows in (1, 100):
 """
     env = dict(os.environ, PYTHONPATH=os.pathsep.join(p for p in sys.path if p))
     subprocess.run([sys.executable, "-c", code], check=True, env=env, timeout=240)
+
+
+@pytest.mark.parametrize("kind,dtype", KIND_TYPES)
+@pytest.mark.parametrize("page", [16, 32, 64, 256])
+def test_attention_of_wide_heads_by_pages(kind, dtype, page):
+    check_attention(ref.Batch(kind, 256, 2, page, [70, 3, 150], [333, 90, 150], seed=page), 4, dtype)
+
+
+@pytest.mark.parametrize("kind,dtype", [("F16", "f16"), ("BF16", "bf16"), ("Q8_0", "bf16"), ("Q4_0", "f16")])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [4, 8, 16, 32, 64, 128])
+@pytest.mark.parametrize("q_lens", [[1, 2], [40, 70]])
+def test_tokens_of_a_page_that_is_not_there_are_left_out(kind, dtype, dim, page, q_lens):
+    """Without a causal mask the result is that of the other pages' tokens."""
+    batch = ref.Batch(kind, dim, 2, page, q_lens, [150, 400], seed=page + dim)
+    batch.poison()
+    q, cache = make_q(batch, 4, dtype), batch.cache(ops)
+    table, start, kv_len = batch.on_gpu()
+    table[1, 1] = batch.k.shape[0]
+    got = ops.paged_attention(q, cache, table, start, kv_len, causal=False).cpu().double()
+    assert mmvq.take_device_status() == ops.BAD_PAGE
+    batch.table[1, 1:-1] = batch.table[1, 2:].clone()
+    batch.kv_lens[1] -= page
+    want, tol = ref.attention(batch, q.cpu(), dim ** -0.5, False)
+    assert ((got - want).abs() <= tol).all()
