@@ -227,12 +227,12 @@ def kv_read(cache: PagedKVCache, page_table: torch.Tensor, start: torch.Tensor, 
     b.kv_len = None
     shape = (rows, cache.kv_heads, cache.head_dim)
     if out is None:
-        out = torch.empty((2,) + shape, dtype=dtype, device=cache.device).unbind(0)  # one allocation
-    else:
-        for t in out:
-            if t.shape != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous() or \
-                    t.data_ptr() % 16:
-                raise _bad(f"out is two contiguous 16-byte aligned {dtype} tensors {shape} on the cache's device")
+        out = (torch.empty(shape, dtype=dtype, device=cache.device),
+               torch.empty(shape, dtype=dtype, device=cache.device))
+    for t in out:
+        if t.shape != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous() or \
+                t.data_ptr() % 16:
+            raise _bad(f"out is two contiguous 16-byte aligned {dtype} tensors {shape} on the cache's device")
     _call(cache, _native.lib().anvil_kv_read, cache._ref, ctypes.byref(b),
           first.data_ptr() if first is not None else None, DTYPES[dtype], out[0].data_ptr(), out[1].data_ptr())
     return out
