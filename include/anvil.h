@@ -434,7 +434,8 @@ int anvil_kv_read(const anvil_kv_cache *cache, const anvil_kv_batch *batch, cons
  * or bf16, with fp32 sums; q of a quantised cache is scaled by a power of two into
  * fp16's range.  workspace: anvil_paged_attention_workspace(cache, batch, heads) bytes of
  * scratch for this call (it depends on batch, total, max_pages and heads alone, not on the
- * lengths), 32-byte aligned; calls that may overlap need their own. */
+ * lengths), 32-byte aligned; calls that may overlap need their own.  Nothing is written outside those
+ * bytes: where they are 0, workspace is not used, null or not. */
 int64_t anvil_paged_attention_workspace(const anvil_kv_cache *cache, const anvil_kv_batch *batch, int heads);
 int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv_batch *batch, int dtype, const void *q,
                           int64_t q_row_stride, int64_t q_head_stride, int heads, float scale, int causal,

@@ -106,8 +106,10 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
     if (p.bytes && (!workspace || workspace_bytes < p.bytes))
         return fail(ANVIL_ERR_INVALID, "a workspace of %lld bytes is needed, got %lld", (long long)p.bytes,
                     (long long)(workspace ? workspace_bytes : 0));
+    // (the kernels write notes wherever there is a place for parts, so a call without joins has none, whatever the
+    // caller's pointer)
     AttnIO io{q, q_row_stride, q_head_stride, out, heads, 0, 0, 0, scale * 1.4426950408889634f,
-              causal != 0, dtype == kKvBF16, static_cast<float *>(workspace)};
+              causal != 0, dtype == kKvBF16, p.join ? static_cast<float *>(workspace) : nullptr};
     set_group(io, heads / cv.kv_heads);
     if (!p.nt)
         return attn_tile_launch(cache->kind, cache->head_dim, cv, bv, io, p.ctas, p.join,

@@ -669,3 +669,53 @@ def test_tokens_of_a_page_that_is_not_there_are_left_out(kind, dtype, dim, page,
     batch.kv_lens[1] -= page
     want, tol = ref.attention(batch, q.cpu(), dim ** -0.5, False)
     assert ((got - want).abs() <= tol).all()
+
+
+# ---- the C entry as a host calls it ------------------------------------------------------------
+
+def c_attention(q, cache, table, start, kv_len, out, work, nbytes, causal=1):
+    import ctypes
+
+    from kernel_anvil import _native
+
+    b = ops._batch(cache, table, start, kv_len, q.shape[0])
+    lib, ref_b = _native.lib(), ctypes.byref(b)
+    need = lib.anvil_paged_attention_workspace(cache._ref, ref_b, q.shape[1])
+    status = lib.anvil_paged_attention(cache._ref, ref_b, ops.DTYPES[q.dtype], q.data_ptr(), q.stride(0), q.stride(1),
+                                       q.shape[1], cache.head_dim ** -0.5, causal, out.data_ptr(), work, nbytes,
+                                       torch.cuda.current_stream().cuda_stream)
+    return need, status
+
+
+@pytest.mark.parametrize("kind,dtype", [("Q8_0", "bf16"), ("F16", "f16")])
+@pytest.mark.parametrize("q_lens", [[1, 2, 1], [40, 50, 64]])           # the rows kernel, the tile kernel
+def test_a_workspace_that_is_not_needed_is_not_written(kind, dtype, q_lens):
+    """Tables of 64 tokens at most need no workspace; a pointer that the host passes all the same stays untouched."""
+    batch = ref.Batch(kind, 128, 2, 16, q_lens, [64, 50, 64], seed=40)
+    cache, q = batch.cache(ops), make_q(batch, 8, dtype)
+    table, start, kv_len = batch.on_gpu()
+    assert table.shape[1] * 16 <= 64
+    want = ops.paged_attention(q, cache, table, start, kv_len)
+    scratch = torch.full((1 << 26,), 0x5A, dtype=torch.uint8, device="cuda")   # notes would lie within it
+    for nbytes in (0, 1024):
+        out = torch.empty_like(want)
+        need, status = c_attention(q, cache, table, start, kv_len, out, scratch.data_ptr() + (1 << 25), nbytes)
+        assert (need, status) == (0, 0)
+        assert torch.equal(out, want)
+        assert bool((scratch == 0x5A).all())
+
+
+@pytest.mark.parametrize("q_lens", [[1, 2], [40, 50]])
+def test_the_workspace_is_as_large_as_asked_for(q_lens):
+    """Exactly the bytes that the query names are written, none before or behind them."""
+    batch = ref.Batch("Q8_0", 128, 2, 16, q_lens, [700, 450], seed=41)
+    cache, q = batch.cache(ops), make_q(batch, 8, "bf16")
+    table, start, kv_len = batch.on_gpu()
+    want = ops.paged_attention(q, cache, table, start, kv_len)
+    need, _ = c_attention(q, cache, table, start, kv_len, torch.empty_like(want), None, 0)
+    assert need > 0
+    scratch = torch.full((need + 8192,), 0x5A, dtype=torch.uint8, device="cuda")
+    out = torch.empty_like(want)
+    assert c_attention(q, cache, table, start, kv_len, out, scratch.data_ptr() + 4096, need) == (need, 0)
+    assert torch.equal(out, want)
+    assert bool((scratch[:4096] == 0x5A).all()) and bool((scratch[4096 + need:] == 0x5A).all())
