@@ -413,7 +413,8 @@ typedef struct anvil_kv_batch {
  * fp16(M / 127); Q4_0 with d = -top / 8 (top: the value of magnitude M, the first of equals)
  * nibble = min(15, floor(x / d + 8.5)), scale fp16(d): the GGUF types' rules.  Magnitudes
  * above 65024 (infinity too) are stored as 65024 there; a block with a NaN reads back as NaN.
- * Two rows at one position: what is stored there is undefined. */
+ * A sequence whose length or starts are out of range is not written at all: a cut entry would name
+ * positions of other tokens.  Two rows at one position: what is stored there is undefined. */
 int anvil_kv_write(const anvil_kv_cache *cache, const anvil_kv_batch *batch, int dtype, const void *k,
                    int64_t k_row_stride, int64_t k_head_stride, const void *v, int64_t v_row_stride,
                    int64_t v_head_stride, anvil_stream_t stream);

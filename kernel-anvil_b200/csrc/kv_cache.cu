@@ -320,10 +320,11 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(KvCacheView c, KvB
         Vec8<T>::load(io.v, t * io.v_row + h * io.v_head + l * 8, v);
         const int b = seq_of_row(bt, int(t));
         if (b >= 0) {
+            // (cut entries would name other positions, with tokens that are to stay)
             const KvSeq s = load_seq(bt, c, b);
             const int pos = s.kv - (s.q1 - s.q0) + (int(t) - s.q0);
-            if (pos >= 0) row = kv_lookup(bt, c, b, pos, h);
-            if ((row < 0 || s.bad) && l == 0) flag_bad_page();
+            if (pos >= 0 && !s.bad) row = kv_lookup(bt, c, b, pos, h);
+            if (row < 0 && l == 0) flag_bad_page();
         }
     }
     store_row<KIND, D>(c.k, c.ks, row, l, k);

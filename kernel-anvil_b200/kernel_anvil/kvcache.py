@@ -201,7 +201,8 @@ def kv_write(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, page_table: 
 
     k, v: (rows, kv_heads, head_dim), float32 / float16 / bfloat16, any row and head strides.  Row i of
     sequence b goes to position kv_len[b] - (q_start[b+1] - q_start[b]) + i.  Rows behind
-    q_start[-1] are left out.  Positions that two sequences of one call share (a common page) must not be
+    q_start[-1] are left out, and so is a sequence with an entry out of range: no cached token is lost to
+    one.  Positions that two sequences of one call share (a common page) must not be
     among those written: both would write them.  The codes are those of the GGUF type for exact arithmetic
     (include/anvil.h); F16 and BF16 round.
     """

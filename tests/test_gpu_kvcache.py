@@ -719,3 +719,39 @@ def test_the_workspace_is_as_large_as_asked_for(q_lens):
     assert c_attention(q, cache, table, start, kv_len, out, scratch.data_ptr() + 4096, need) == (need, 0)
     assert torch.equal(out, want)
     assert bool((scratch[:4096] == 0x5A).all()) and bool((scratch[4096 + need:] == 0x5A).all())
+
+
+# ---- entries out of range, rows of no sequence -------------------------------------------------
+
+BAD_LENS = [[65, 33], [1000, 33], [2 ** 31 - 1, 33], [-5, 33], [64, -1], [-2 ** 31, 2 ** 31 - 1]]
+BAD_STARTS = [[0, 2, 99], [-1, 2, 3], [0, 2 ** 31 - 1, 3], [-2 ** 31, 2, 3]]
+
+
+@pytest.mark.parametrize("kind,dtype", [("Q8_0", "f32"), ("Q4_0", "bf16"), ("F16", "f16")])
+def test_a_write_with_bad_lengths_or_starts_changes_no_other_token(kind, dtype):
+    """A sequence with an entry out of range is not written: its cached tokens, and all others, stay bit for bit."""
+    batch = ref.Batch(kind, 64, 2, 16, [2, 1], [64, 33], seed=42)
+    cache = batch.cache(ops)
+    table, start, kv_len = batch.on_gpu()
+    assert table.shape[1] * 16 == 64
+    new = torch.randn(3, 2, 64, generator=batch.gen).to(ref.NP[dtype]).cuda()
+    tensors = [t for t in (cache.k, cache.v, cache.k_scale, cache.v_scale) if t is not None]
+    before = [t.clone() for t in tensors]
+    calls = [(lens, [0, 2, 3]) for lens in BAD_LENS] + [([64, 33], s) for s in BAD_STARTS] + [([70, 130], [0, 2, 99])]
+    for lens, starts in calls:
+        ops.kv_write(cache, new, new, table, torch.tensor(starts, dtype=torch.int32).cuda(),
+                     torch.tensor(lens, dtype=torch.int32).cuda())
+        assert mmvq.take_device_status() == ops.BAD_PAGE, (lens, starts)
+        for b, n in enumerate(batch.kv_lens):           # the sequences whose entries are all in range are written
+            a, z = starts[b], starts[b + 1]
+            fine = 0 <= a <= z <= 3 and 0 <= lens[b] <= 64
+            p, o = batch.slots(b, torch.arange(n))
+            own = torch.arange(n) >= (n - (z - a) if fine else n)
+            for t, was in zip(tensors, before):
+                got, old = t[p.cuda(), :, o.cuda()].cpu(), was[p.cuda(), :, o.cuda()].cpu()
+                assert torch.equal(got[~own], old[~own]), (lens, starts, b)
+                assert not own.any() or not torch.equal(got[own], old[own])
+        for t, was in zip(tensors, before):
+            t.copy_(was)
+    ops.kv_write(cache, new, new, table, start, kv_len)
+    assert mmvq.take_device_status() == 0
