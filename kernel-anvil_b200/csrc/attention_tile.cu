@@ -556,8 +556,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if constexpr (!S::quant) {
             // 16-bit rows go straight to their places: from pages of 8 keys and more by TMA, boxes of up to 64 keys of one
             // page and 64 columns; from smaller ones by cp.async, a tile announced when the next one's copies are on their way.
-            // Of a tile that some row does not see whole, or that lacks pages, what is not finite and what is no key
-            // leaves the values first (see the outputs).
+            // Of a tile that lacks pages, or keys behind the last, what is no key leaves the values first; of one that some row
+            // does not see whole, what is not finite too (the outputs bring it back to the rows that see it).
             constexpr int CH = D / 8;
             auto clean = [&](const TileUnit<KIND, D> &u, int t, int b, int from) {  // by threads `from` and up
                 const int left = u.key_end - t * S::keys;
@@ -568,6 +568,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
                         if (r >= left || ((bad[r >> 5] >> (r & 31)) & 1))
                             *reinterpret_cast<uint4 *>(place(1, b, r, ch)) = make_uint4(0, 0, 0, 0);
                 }
+                if ((t + 1) * S::keys <= u.free_end) return;  // only a page was missing: every row sees the other keys
                 // 0 x value summed: NaN if any value is not finite
                 uint32_t odd = 0;
 #pragma unroll 4

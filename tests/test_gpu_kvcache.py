@@ -755,3 +755,31 @@ def test_a_write_with_bad_lengths_or_starts_changes_no_other_token(kind, dtype):
             t.copy_(was)
     ops.kv_write(cache, new, new, table, start, kv_len)
     assert mmvq.take_device_status() == 0
+
+
+@pytest.mark.parametrize("kind,dtype", [("F16", "f16"), ("BF16", "bf16"), ("Q8_0", "f16"), ("Q4_0", "bf16")])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [4, 8, 16, 32])
+@pytest.mark.parametrize("q_lens", [[1, 2], [40, 70]])
+def test_a_value_beside_a_page_that_is_not_there_still_counts(kind, dtype, dim, page, q_lens):
+    """An infinite value in a tile that every row sees whole but for a missing page; NaN in the masked ones."""
+    batch = ref.Batch(kind, dim, 2, page, q_lens, [150, 400], seed=page + dim)
+    p, o = batch.slots(1, 3)
+    if batch.vs is None:
+        batch.v[p, 0, o, 5] = float("inf")
+    else:
+        batch.vs[p, 0, o, 1] = float("nan")
+    q, cache = make_q(batch, 4, dtype), batch.cache(ops)
+    table, start, kv_len = batch.on_gpu()
+    table[1, 1] = -1
+    for causal in (False, True):                 # (the early tile is seen whole in both)
+        got = ops.paged_attention(q, cache, table, start, kv_len, causal=causal).cpu()
+        assert mmvq.take_device_status() == ops.BAD_PAGE
+        rows = got[q_lens[0]:, :2]               # query heads 0 and 1 read key/value head 0
+        if batch.vs is None:
+            assert (rows[..., 5] == float("inf")).all()
+            assert torch.isfinite(rows[..., :5]).all() and torch.isfinite(rows[..., 6:]).all()
+        else:
+            assert torch.isnan(rows[..., 32:64]).all()
+            assert torch.isfinite(rows[..., :32]).all() and torch.isfinite(rows[..., 64:]).all()
+        assert torch.isfinite(got[:q_lens[0]]).all() and torch.isfinite(got[:, 2:]).all()
