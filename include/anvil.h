@@ -383,7 +383,7 @@ int anvil_ipc_free(void *ptr);
  * A cache holds one layer: k and v are (num_pages, kv_heads, page_size, row), row-major, where a
  * row is head_dim values of `kind` (ggml type ids):
  *   1 F16, 30 BF16: 16-bit values; k_scale = v_scale = NULL.
- *   8 Q8_0: int8 codes.  2 Q4_0: head_dim / 2 bytes, nibbles in GGUF order (value e < 16 of
+ *   8 Q8_0: int8 codes, -127..127.  2 Q4_0: head_dim / 2 bytes, nibbles in GGUF order (value e < 16 of
  *   a 32-value block in the low nibble of its byte e, e >= 16 in the high nibble of byte
  *   e - 16; nibble - 8).  The scales (fp16, one per 32 values) are k_scale and v_scale,
  *   (num_pages, kv_heads, page_size, head_dim / 32).
@@ -433,7 +433,9 @@ int anvil_kv_read(const anvil_kv_cache *cache, const anvil_kv_batch *batch, cons
  * lies behind kv_len in a page is never used; keys that a row does not see do not reach it, NaN
  * and infinities among them.  Products run on the tensor cores in fp16 (F16 and quantised caches)
  * or bf16, with fp32 sums; q of a quantised cache is scaled by a power of two into
- * fp16's range.  workspace: anvil_paged_attention_workspace(cache, batch, heads) bytes of
+ * fp16's range.  There a block whose scale is above 512 (Q8_0) or 8188 (Q4_0) in magnitude, so that
+ * values could pass fp16's range, counts as NaN; anvil_kv_write stores none, and anvil_kv_read
+ * gives its values.  workspace: anvil_paged_attention_workspace(cache, batch, heads) bytes of
  * scratch for this call (it depends on batch, total, max_pages and heads alone, not on the
  * lengths), 32-byte aligned; calls that may overlap need their own.  Nothing is written outside those
  * bytes: where they are 0, workspace is not used, null or not. */

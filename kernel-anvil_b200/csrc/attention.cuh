@@ -328,22 +328,6 @@ template <bool BF16> __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) 
     return ((w & E) == E ? 0xFFFFu : 0u) | (((w >> 16) & E) == E ? 0xFFFF0000u : 0u);
 }
 
-// Value e of a cache row.
-template <int KIND, int D>
-__device__ __forceinline__ float kv_value(const uint8_t *data, const __half *scales, int64_t row, int e) {
-    if constexpr (KIND == kKvF16) {
-        return __half2float(reinterpret_cast<const __half *>(data)[row * D + e]);
-    } else if constexpr (KIND == kKvBF16) {
-        return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(data)[row * D + e]);
-    } else if constexpr (KIND == kKvQ8_0) {
-        return float(reinterpret_cast<const int8_t *>(data)[row * D + e]) *
-               __half2float(scales[row * (D / 32) + e / 32]);
-    } else {
-        const uint8_t w = data[row * (D / 2) + (e / 32) * 16 + (e % 16)];
-        return float(int((e % 32) < 16 ? w & 15 : w >> 4) - 8) * __half2float(scales[row * (D / 32) + e / 32]);
-    }
-}
-
 __device__ __forceinline__ uint32_t h2sub(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -360,6 +344,38 @@ __device__ __forceinline__ uint32_t h2fma(uint32_t a, uint32_t b, uint32_t c) {
     return r;
 }
 __device__ __forceinline__ uint32_t dup16(uint32_t x) { return __byte_perm(x, x, 0x1010); }
+
+// Two blocks' scales as the products take them: NaN where a block's largest value could pass fp16, above 512 (Q8_0, codes
+// of up to 127) or 8188 (Q4_0, of up to 8), which a cache that anvil_kv_write filled does not have.  Products of such
+// scales would be infinite in some places only, and zero weights times them NaN in rows that do not see them; so the block is
+// one with a non-finite scale, of which the kernels take care.  The largest allowed scale times the factor is 65504, the
+// next one's product rounds to infinity, and zero times that is NaN.
+template <int KIND> __device__ __forceinline__ uint32_t usable_scales(uint32_t d) {
+    constexpr uint32_t factor = KIND == kKvQ8_0 ? 0x57FF57FFu : 0x48004800u;  // 127.9375, 8
+    return h2fma(h2mul(d, factor), 0u, d);
+}
+// From here on, in bits of the magnitude, a usable scale needs care in tiles that some row does not see: NaN; and 512, which
+// with the code -128 (not of the type, but a tensor may hold it) passes fp16, while 511.75, 2^-11 less, does not.
+template <int KIND> constexpr uint32_t kOddScale = KIND == kKvQ8_0 ? 0x6000 : 0x7C00;
+
+// Value e of a cache row, as the products take it.
+template <int KIND, int D>
+__device__ __forceinline__ float kv_value(const uint8_t *data, const __half *scales, int64_t row, int e) {
+    auto scale = [&] {
+        const uint32_t d = usable_scales<KIND>(__half_as_ushort(scales[row * (D / 32) + e / 32]));
+        return __half2float(__ushort_as_half(uint16_t(d)));
+    };
+    if constexpr (KIND == kKvF16) {
+        return __half2float(reinterpret_cast<const __half *>(data)[row * D + e]);
+    } else if constexpr (KIND == kKvBF16) {
+        return __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(data)[row * D + e]);
+    } else if constexpr (KIND == kKvQ8_0) {
+        return float(reinterpret_cast<const int8_t *>(data)[row * D + e]) * scale();
+    } else {
+        const uint8_t w = data[row * (D / 2) + (e / 32) * 16 + (e % 16)];
+        return float(int((e % 32) < 16 ? w & 15 : w >> 4) - 8) * scale();
+    }
+}
 
 // Joins the partial results of the unit that CTA `blockIdx.x` of the attention kernel began and did
 // not finish: o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p.  A row's parts are shared by 1, 2, 4 or 8 of the

@@ -338,6 +338,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
 #pragma unroll
                         for (int j = 0; j < NB / 4; ++j)
                             *reinterpret_cast<uint2 *>(&dw[i][2 * j]) = *reinterpret_cast<const uint2 *>(at + 4 * j);
+#pragma unroll
+                    for (int j = 0; j < NB / 2; ++j) dw[i][j] = usable_scales<KIND>(dw[i][j]);
                 }
 #pragma unroll
                 for (int b = 0; b < NB; ++b) {
@@ -361,10 +363,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                     }
                     float d[2];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float y = __half2float(__ushort_as_half(uint16_t(dw[i][b >> 1] >> (16 * (b & 1)))));
-                        d[i] = fmaf(0.0f, y, y);  // an infinite scale is NaN, as zero codes times it are
-                    }
+                    for (int i = 0; i < 2; ++i)
+                        d[i] = __half2float(__ushort_as_half(uint16_t(dw[i][b >> 1] >> (16 * (b & 1)))));
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -448,8 +448,10 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                 if constexpr (S::quant) {
                     if (lane < 16)
 #pragma unroll
-                        for (int i = 0; i < D / 32; ++i)
-                            odd |= nonfinite2<false>(__half_as_ushort(vs[lane * (D / 32) + i])) != 0;
+                        for (int i = 0; i < D / 32; ++i) {
+                            const uint32_t y = usable_scales<KIND>(__half_as_ushort(vs[lane * (D / 32) + i]));
+                            odd |= (y & 0x7FFFu) >= kOddScale<KIND>;
+                        }
                 } else {
                     for (int i = lane; i < kRowsStep * S::ch; i += 32) {
                         const uint4 w = *reinterpret_cast<const uint4 *>(sv + (i / S::ch) * S::vst + (i % S::ch) * 16);
@@ -466,7 +468,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                                 const int at = KIND == kKvQ4_0 ? (dim / 32) * 16 + (dim & 15) : S::quant ? dim : 2 * dim;
                                 const uint8_t *b = sv + k * S::vst + at;
                                 float x;
-                                if constexpr (S::quant) x = __half2float(vs[k * (D / 32) + dim / 32]);
+                                if constexpr (S::quant)
+                                    x = __half2float(__ushort_as_half(
+                                        uint16_t(usable_scales<KIND>(__half_as_ushort(vs[k * (D / 32) + dim / 32])))));
                                 else if constexpr (BF) x = __uint_as_float(uint32_t(*reinterpret_cast<const uint16_t *>(b)) << 16);
                                 else x = __half2float(*reinterpret_cast<const __half *>(b));
                                 if constexpr (KIND == kKvQ8_0) x *= float(*reinterpret_cast<const int8_t *>(b));
@@ -481,8 +485,11 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                         }
                     __syncwarp();
                     if constexpr (S::quant) {
-                        for (int i = lane; i < kRowsStep * (D / 32); i += 32)
-                            if (nonfinite2<false>(__half_as_ushort(vs[i]))) vs[i] = __ushort_as_half(0);
+                        for (int i = lane; i < kRowsStep * (D / 32); i += 32) {
+                            const uint32_t y = usable_scales<KIND>(__half_as_ushort(vs[i]));
+                            if ((y & 0x7FFFu) >= kOddScale<KIND>)
+                                vs[i] = __ushort_as_half(uint16_t(KIND == kKvQ8_0 && (y & 0x7FFFu) == 0x6000u ? y - 1 : 0));
+                        }
                     } else {
                         for (int i = lane; i < kRowsStep * S::ch * 4; i += 32) {
                             uint32_t *w = reinterpret_cast<uint32_t *>(sv + (i / (4 * S::ch)) * S::vst + (i % (4 * S::ch)) * 4);
@@ -505,8 +512,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
                 uint32_t h[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) h[j] = __half_as_ushort(vs[r4[j] * (D / 32) + dim / 32]);
-                d01 = h[0] | (h[1] << 16);
-                d23 = h[2] | (h[3] << 16);
+                d01 = usable_scales<KIND>(h[0] | (h[1] << 16));
+                d23 = usable_scales<KIND>(h[2] | (h[3] << 16));
             };
             auto q8_word = [&](int i, const uint32_t (&w)[4]) {  // 4 owned dimensions: tiles i, i + 1
 #pragma unroll

@@ -77,7 +77,11 @@ class PagedKVCache:
     @classmethod
     def from_buffers(cls, kind: str, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                      v_scale: torch.Tensor | None = None) -> "PagedKVCache":
-        """A cache on tensors that the caller holds (used in place)."""
+        """A cache on tensors that the caller holds (used in place).
+
+        Scales above 512 (Q8_0) or 8188 (Q4_0) in magnitude, which kv_write never makes, pass fp16's range with
+        their codes: paged_attention takes such a block as NaN, kv_read gives its values.
+        """
         self = cls.__new__(cls)
         self._take(kind, k, v, k_scale, v_scale)
         return self

@@ -783,3 +783,83 @@ def test_a_value_beside_a_page_that_is_not_there_still_counts(kind, dtype, dim, 
             assert torch.isnan(rows[..., 32:64]).all()
             assert torch.isfinite(rows[..., :32]).all() and torch.isfinite(rows[..., 64:]).all()
         assert torch.isfinite(got[:q_lens[0]]).all() and torch.isfinite(got[:, 2:]).all()
+
+
+# ---- scales beyond what the products carry -------------------------------------------------------
+
+def set_block(batch, name, b, pos, scale, code):
+    """One cached token's scales and codes, all alike."""
+    p, o = batch.slots(b, pos)
+    codes, scales = (batch.k, batch.ks) if name == "k" else (batch.v, batch.vs)
+    scales[p, :, o] = scale
+    codes[p, :, o] = code
+
+
+@pytest.mark.parametrize("kind,scale,code", [("Q8_0", 516.0, 127), ("Q8_0", 6.0e4, 1), ("Q8_0", -512.5, -127),
+                                             ("Q8_0", -600.0, 0), ("Q4_0", 8192.0, 0x00), ("Q4_0", -3.0e4, 0x99)])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 4), (128, 64), (256, 16)])
+@pytest.mark.parametrize("q_lens", [[4, 5, 12], [40, 5, 150]])
+def test_a_scale_beyond_the_range_reaches_only_the_rows_that_see_it(kind, scale, code, dim, page, q_lens):
+    """A finite scale above 512 (Q8_0) or 8188 (Q4_0) counts as NaN for the rows that see its token, in keys and
+    values, and does not reach the others; it reads back as the value that it stands for."""
+    kv_lens, at = [70, 30, 400], {0: 68, 1: 27, 2: 395}
+    if q_lens[2] == 150:
+        at[2] = 300
+    for name in "kv":
+        batch = ref.Batch(kind, dim, 1, page, q_lens, kv_lens, seed=43)
+        clean = ref.Batch(kind, dim, 1, page, q_lens, kv_lens, seed=43)
+        for b, pos in at.items():
+            set_block(batch, name, b, pos, scale, code)
+        q = make_q(batch, 2, "f16")
+        cache, (table, start, kv_len) = batch.cache(ops), batch.on_gpu()
+        got = ops.paged_attention(q, cache, table, start, kv_len).cpu().double()
+        want, tol = ref.attention(clean, q.cpu(), dim ** -0.5, True)
+        for b, pos in at.items():
+            n, kv, t0 = q_lens[b], kv_lens[b], int(batch.start[b])
+            blind = pos - (kv - n)                      # rows 0 .. blind-1 stand before it
+            assert 0 < blind < n
+            assert ((got - want).abs() <= tol)[t0:t0 + blind].all(), (name, b)
+            assert torch.isnan(got[t0 + blind:t0 + n]).all(), (name, b)
+        rows = torch.tensor([0, 0, 0, 400], dtype=torch.int32).cuda()
+        read = ops.kv_read(cache, table, rows, 400)["kv".index(name)]
+        assert torch.equal(read.cpu(), batch.rows_of(name, 2).float())
+
+
+@pytest.mark.parametrize("kind,scale,codes", [("Q8_0", 512.0, (127, -127)), ("Q4_0", -8188.0, (0x00, 0xFF))])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q_lens", [[4, 5], [40, 150]])
+def test_the_largest_scales_are_ordinary_ones(kind, scale, codes, dim, q_lens):
+    """Values of up to 65504 in some tokens, beside ordinary ones.
+
+    Where some row does not see a tile, 512 is taken as 511.75, 2^-11 of it less: A 2^-11 more than the bound, which has
+    A (u_p + u_v) = A 2^-10 in it, so half of the bound more.
+    """
+    batch = ref.Batch(kind, dim, 1, 16, q_lens, [70, 400], seed=44)
+    for i, pos in enumerate((20, 66, 69)):
+        set_block(batch, "v", 0, pos, scale, codes[i & 1])
+        set_block(batch, "v", 1, pos * 5, scale, codes[i & 1])
+    q = make_q(batch, 2, "f16")
+    table, start, kv_len = batch.on_gpu()
+    for factor in (0.01, 1e-6):
+        want, tol = ref.attention(batch, q.cpu(), factor, True)
+        got = ops.paged_attention(q, batch.cache(ops), table, start, kv_len, scale=factor).cpu().double()
+        assert ((got - want).abs() <= tol * (1.5 if kind == "Q8_0" else 1)).all()
+        set_block(batch, "k", 0, 31, scale, codes[0])
+        set_block(batch, "k", 1, 31, scale, codes[1])
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 4), (256, 16)])
+@pytest.mark.parametrize("q_lens", [[4, 12], [40, 150]])
+def test_the_code_that_no_write_makes_stays_with_the_rows_that_see_it(dim, page, q_lens):
+    """-128 (outside the type's codes) times the largest scale passes fp16's range."""
+    batch, clean = (ref.Batch("Q8_0", dim, 1, page, q_lens, [70, 400], seed=45) for _ in range(2))
+    at = {0: 68, 1: 395 if q_lens[1] == 12 else 300}
+    for b, pos in at.items():
+        set_block(batch, "v", b, pos, 512.0 - 1024.0 * b, -128)
+    q = make_q(batch, 2, "f16")
+    table, start, kv_len = batch.on_gpu()
+    got = ops.paged_attention(q, batch.cache(ops), table, start, kv_len).cpu().double()
+    want, tol = ref.attention(clean, q.cpu(), dim ** -0.5, True)
+    for b, pos in at.items():
+        t0, blind = int(batch.start[b]), pos - (batch.kv_lens[b] - q_lens[b])
+        assert ((got - want).abs() <= tol)[t0:t0 + blind].all(), b
