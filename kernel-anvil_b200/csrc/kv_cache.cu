@@ -305,6 +305,14 @@ __device__ __forceinline__ int seq_of_row(const KvBatchView &bt, int t) {
     return bt.start[lo] <= t && t < bt.start[lo + 1] ? lo : -1;
 }
 
+// By the grid's first CTA: reports every start and length out of range, of sequences without rows in this call too.
+__device__ __forceinline__ void report_bad_entries(const KvCacheView &c, const KvBatchView &bt) {
+    if (blockIdx.x || blockIdx.y) return;
+    bool bad = false;
+    for (int b = threadIdx.x; b < bt.batch; b += blockDim.x) bad |= load_seq(bt, c, b).bad;
+    if (bad) flag_bad_page();
+}
+
 constexpr int kKvThreads = 256;
 
 template <typename T, int KIND, int D>
@@ -329,6 +337,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_write_kernel(KvCacheView c, KvB
     }
     store_row<KIND, D>(c.k, c.ks, row, l, k);
     store_row<KIND, D>(c.v, c.vs, row, l, v);
+    report_bad_entries(c, bt);
 }
 
 template <typename T, int KIND, int D>
@@ -336,6 +345,7 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(KvCacheView c, KvBa
     constexpr int LPR = D / 8;
     const int64_t t = int64_t(blockIdx.x) * (kKvThreads / LPR) + threadIdx.x / LPR;
     const int l = threadIdx.x % LPR, h = blockIdx.y;
+    report_bad_entries(c, bt);
     if (t >= bt.total) return;
     const int b = seq_of_row(bt, int(t));
     if (b < 0) return;  // a row behind the last sequence
@@ -459,6 +469,7 @@ extern "C" int anvil_kv_read(const anvil_kv_cache *cache, const anvil_kv_batch *
     KvCacheView cv;
     KvBatchView bv;
     if (int s = kv_check(cache, batch, &cv, &bv)) return s;
+    bv.kv_len = nullptr;  // lengths are no part of a read
     if (bv.batch && bv.total) {
         if (!k || !v) return fail(ANVIL_ERR_INVALID, "null k or v");
         if (!aligned(k, 16) || !aligned(v, 16) || !aligned(first, 4))

@@ -863,3 +863,48 @@ def test_the_code_that_no_write_makes_stays_with_the_rows_that_see_it(dim, page,
     for b, pos in at.items():
         t0, blind = int(batch.start[b]), pos - (batch.kv_lens[b] - q_lens[b])
         assert ((got - want).abs() <= tol)[t0:t0 + blind].all(), b
+
+
+def test_starts_and_lengths_out_of_range_are_reported_by_write_and_read():
+    batch = ref.Batch("Q8_0", 64, 2, 16, [3, 0, 2], [40, 20, 33], seed=46)
+    cache = batch.cache(ops)
+    table, start, kv_len = batch.on_gpu()
+    new = torch.randn(5, 2, 64, device="cuda")
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32).cuda()  # noqa: E731
+    write = lambda s, n: ops.kv_write(cache, new, new, table, s, n)  # noqa: E731
+    read = lambda s, n: ops.kv_read(cache, table, s, 5)  # noqa: E731
+    for call in (write, read):
+        call(start, kv_len)
+        assert mmvq.take_device_status() == 0
+        for s in ([0, 5, 3, 5], [0, 5, 5, 3], [0, 3, 3, 99], [-1, 3, 3, 5], [0, 3, -7, 5], [2 ** 31 - 1, -2 ** 31, 0, 0],
+                  [6, 6, 6, 6], [-3, -2, -1, 0]):
+            call(i32(s), kv_len)
+            assert mmvq.take_device_status() == ops.BAD_PAGE, s
+    for lens in ([40, 65, 33], [40, -1, 33], [40, 2 ** 31 - 1, 33]):   # of a sequence without new tokens
+        write(start, i32(lens))
+        assert mmvq.take_device_status() == ops.BAD_PAGE, lens
+    # many sequences, of which one of the last has the bad entry
+    many = torch.arange(2001, dtype=torch.int32, device="cuda").clamp(max=5)
+    pages, lens = table[:1].expand(2000, -1).contiguous(), torch.full((2000,), 20, dtype=torch.int32, device="cuda")
+    for call in (lambda s: ops.kv_write(cache, new, new, pages, s, lens), lambda s: ops.kv_read(cache, pages, s, 5)):
+        call(many)
+        assert mmvq.take_device_status() == 0
+        late = many.clone()
+        late[1990] = 4
+        call(late)
+        assert mmvq.take_device_status() == ops.BAD_PAGE
+
+
+def test_a_read_does_not_look_at_the_lengths():
+    import ctypes
+
+    from kernel_anvil import _native
+
+    batch = ref.Batch("Q8_0", 64, 2, 16, [3, 2], [40, 33], seed=51)
+    cache, (table, start, kv_len) = batch.cache(ops), batch.on_gpu()
+    b = ops._batch(cache, table, start, kv_len - 2 ** 30, 5)
+    k, v = torch.empty(2, 5, 2, 64, device="cuda")
+    assert _native.lib().anvil_kv_read(cache._ref, ctypes.byref(b), None, 0, k.data_ptr(), v.data_ptr(),
+                                       torch.cuda.current_stream().cuda_stream) == 0
+    assert mmvq.take_device_status() == 0
+    assert torch.equal(v[:3].cpu(), batch.rows_of("v", 0, 3).float())
