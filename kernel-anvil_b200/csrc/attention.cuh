@@ -303,13 +303,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// The exponent of 2 that the row of a bf16 query is multiplied by so that it fits fp16 (its
-// largest magnitude in [2^13, 2^14)); 0 for zeros, infinities and NaN.  Bounded so that the
-// factor and its inverse are fp32 numbers.
+// The exponent of 2 that the row of a bf16 query is multiplied by so that it fits fp16: its largest magnitude goes to
+// [2^13, 2^14), as far as the factor and its inverse are normal fp32 numbers, from 2^-114 to 2^126 (which brings the
+// smallest normal magnitude to 1).  0 for zeros, infinities and NaN.
 __device__ __forceinline__ int q_exponent(uint32_t amax_bits) {
     const int e = int(amax_bits >> 23);
     if (amax_bits == 0 || e == 255) return 0;
-    return max(-100, min(100, 127 + 13 - e));
+    return min(126, 127 + 13 - e);
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 

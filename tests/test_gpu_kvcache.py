@@ -908,3 +908,13 @@ def test_a_read_does_not_look_at_the_lengths():
                                        torch.cuda.current_stream().cuda_stream) == 0
     assert mmvq.take_device_status() == 0
     assert torch.equal(v[:3].cpu(), batch.rows_of("v", 0, 3).float())
+
+
+@pytest.mark.parametrize("kind", ["Q8_0", "Q4_0"])
+@pytest.mark.parametrize("q_len", [1, 100])
+def test_queries_at_both_ends_of_bf16_meet_a_scale_that_brings_them_back(kind, q_len):
+    """A quantised cache's queries are brought into fp16's range whatever their exponent."""
+    batch = ref.Batch(kind, 128, 1, 16, [q_len], [300], seed=49)
+    check_attention(batch, 4, "bf16", amp=2.0 ** 122, scale=0.09 * 2.0 ** -122)
+    check_attention(batch, 4, "bf16", amp=2.0 ** 112, scale=0.09 * 2.0 ** -112)
+    check_attention(batch, 4, "bf16", amp=2.0 ** -121, scale=0.09 * 2.0 ** 121)
