@@ -97,7 +97,8 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
         return fail(ANVIL_ERR_UNSUPPORTED, "%d rows of %d heads are too many for one call", bv.total, heads);
     if (bv.batch == 0 || bv.total == 0) return ANVIL_OK;
     if (!q || !out || !bv.kv_len) return fail(ANVIL_ERR_INVALID, "null q, out or kv_len");
-    if (!std::isfinite(scale)) return fail(ANVIL_ERR_INVALID, "scale=%f is not finite", double(scale));
+    const float scale_log2 = scale * 1.4426950408889634f;
+    if (!std::isfinite(scale_log2)) return fail(ANVIL_ERR_INVALID, "scale=%g is not finite in powers of two", double(scale));
     const auto mis = [](const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 != 0; };
     if (mis(q) || mis(out) || q_row_stride % 8 || q_head_stride % 8)
         return fail(ANVIL_ERR_ALIGN, "q, its rows and out must be 16-byte aligned");
@@ -108,7 +109,7 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
                     (long long)(workspace ? workspace_bytes : 0));
     // (the kernels write notes wherever there is a place for parts, so a call without joins has none, whatever the
     // caller's pointer)
-    AttnIO io{q, q_row_stride, q_head_stride, out, heads, 0, 0, 0, scale * 1.4426950408889634f,
+    AttnIO io{q, q_row_stride, q_head_stride, out, heads, 0, 0, 0, scale_log2,
               causal != 0, dtype == kKvBF16, p.join ? static_cast<float *>(workspace) : nullptr};
     set_group(io, heads / cv.kv_heads);
     if (!p.nt)

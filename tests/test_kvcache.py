@@ -144,6 +144,14 @@ def test_c_abi_refuses_null_structs_and_mixed_types():
     assert calls(c_cache(), c_batch(kv_len=None))["attention"]() == ANVIL_ERR_INVALID
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), float("-inf"), 2.9e38, -3.4e38])
+def test_c_abi_refuses_scales_that_are_not_finite(scale):
+    """2.9e38 is finite, but not times log2(e), which the scores are multiplied by."""
+    status = _native.lib().anvil_paged_attention(ctypes.byref(c_cache()), ctypes.byref(c_batch()), 1, 16, 256, 128, 4,
+                                                 scale, 1, 64, 32, 1 << 40, None)
+    assert status == ANVIL_ERR_INVALID and "scale" in _native.last_error()
+
+
 def test_c_abi_empty_calls_do_nothing():
     for b in (c_batch(total=0, start=None, page_table=None), c_batch(batch=0)):
         for name, call in calls(c_cache(), b, k=None, v=None, out=None).items():
