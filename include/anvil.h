@@ -84,7 +84,9 @@ enum anvil_flags {
      * weight tile before it waits for the preceding kernel in the stream, so the
      * weights must not be written by that kernel (true for model weights).
      * Activations and outputs are only touched after the wait. */
-    ANVIL_FLAG_PDL = 1u << 0
+    ANVIL_FLAG_PDL = 1u << 0,
+    /* The cache's read and attention: rows of no sequence are written, with zeros. */
+    ANVIL_FLAG_ZERO_REST = 1u << 1
 };
 
 /* ---- library ------------------------------------------------------------ */
@@ -395,7 +397,8 @@ typedef struct anvil_kv_cache {
 
 /* A ragged batch on the device.  Sequence b has the packed rows start[b] .. start[b+1]-1 of the
  * call's k, v, q and out (start: batch + 1 values, ascending); rows behind start[batch] (of
- * `total`) are neither read nor written.  kv_len[b] tokens of it are in the cache, the new ones
+ * `total`) or before start[0] are of no sequence: not used, and outputs stay as they were there
+ * (unless a call has ANVIL_FLAG_ZERO_REST).  kv_len[b] tokens of it are in the cache, the new ones
  * included: its row i is at position kv_len[b] - (start[b+1] - start[b]) + i.  Position p is in
  * page page_table[b * page_table_stride + p / page_size], p below 2^31 - 4096.  Entries are read on the device: one
  * that is out of range is cut or skipped, never followed, and raises ANVIL_DEVICE_BAD_PAGE. */
@@ -424,6 +427,9 @@ int anvil_kv_write(const anvil_kv_cache *cache, const anvil_kv_batch *batch, int
  * each code * scale rounded once; zeros for a position without a page. */
 int anvil_kv_read(const anvil_kv_cache *cache, const anvil_kv_batch *batch, const int32_t *first, int dtype,
                   void *k, void *v, anvil_stream_t stream);
+/* The same with flags (0 or ANVIL_FLAG_ZERO_REST). */
+int anvil_kv_read_ex(const anvil_kv_cache *cache, const anvil_kv_batch *batch, const int32_t *first, int dtype,
+                     void *k, void *v, unsigned flags, anvil_stream_t stream);
 
 /* out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j over the cached tokens j that the row
  * sees: all kv_len[b] of its sequence, or, causal, those up to its own position; zeros for a
@@ -443,6 +449,11 @@ int64_t anvil_paged_attention_workspace(const anvil_kv_cache *cache, const anvil
 int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv_batch *batch, int dtype, const void *q,
                           int64_t q_row_stride, int64_t q_head_stride, int heads, float scale, int causal,
                           void *out, void *workspace, int64_t workspace_bytes, anvil_stream_t stream);
+/* The same with flags (0 or ANVIL_FLAG_ZERO_REST). */
+int anvil_paged_attention_ex(const anvil_kv_cache *cache, const anvil_kv_batch *batch, int dtype, const void *q,
+                             int64_t q_row_stride, int64_t q_head_stride, int heads, float scale, int causal,
+                             void *out, void *workspace, int64_t workspace_bytes, unsigned flags,
+                             anvil_stream_t stream);
 
 /* ---- smithy runtime config (replaces patches/smithy-config.h) ------------ */
 

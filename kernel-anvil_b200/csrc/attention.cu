@@ -84,6 +84,14 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
                                      const void *q, int64_t q_row_stride, int64_t q_head_stride, int heads,
                                      float scale, int causal, void *out, void *workspace,
                                      int64_t workspace_bytes, anvil_stream_t stream) {
+    return anvil_paged_attention_ex(cache, batch, dtype, q, q_row_stride, q_head_stride, heads, scale, causal, out,
+                                    workspace, workspace_bytes, 0, stream);
+}
+
+extern "C" int anvil_paged_attention_ex(const anvil_kv_cache *cache, const anvil_kv_batch *batch, int dtype,
+                                        const void *q, int64_t q_row_stride, int64_t q_head_stride, int heads,
+                                        float scale, int causal, void *out, void *workspace,
+                                        int64_t workspace_bytes, unsigned flags, anvil_stream_t stream) {
     KvCacheView cv;
     KvBatchView bv;
     if (int s = kv_check(cache, batch, &cv, &bv)) return s;
@@ -95,7 +103,14 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
         return fail(ANVIL_ERR_INVALID, "heads=%d is not a multiple of kv_heads=%d", heads, cv.kv_heads);
     if (int64_t(bv.total) * heads > 0x7fffffff - 1024)
         return fail(ANVIL_ERR_UNSUPPORTED, "%d rows of %d heads are too many for one call", bv.total, heads);
-    if (bv.batch == 0 || bv.total == 0) return ANVIL_OK;
+    if (flags & ~unsigned(ANVIL_FLAG_ZERO_REST)) return fail(ANVIL_ERR_INVALID, "flags=0x%x", flags);
+    if (bv.total == 0 || (bv.batch == 0 && !flags)) return ANVIL_OK;
+    if (bv.batch == 0) {  // all rows are of no sequence
+        if (!out) return fail(ANVIL_ERR_INVALID, "null out");
+        const cudaError_t e = cudaMemsetAsync(out, 0, size_t(bv.total) * heads * cache->head_dim * 2,
+                                              reinterpret_cast<cudaStream_t>(stream));
+        return e == cudaSuccess ? ANVIL_OK : cuda_fail(e, "paged_attention memset");
+    }
     if (!q || !out || !bv.kv_len) return fail(ANVIL_ERR_INVALID, "null q, out or kv_len");
     const float scale_log2 = scale * 1.4426950408889634f;
     if (!std::isfinite(scale_log2)) return fail(ANVIL_ERR_INVALID, "scale=%g is not finite in powers of two", double(scale));
@@ -110,7 +125,7 @@ extern "C" int anvil_paged_attention(const anvil_kv_cache *cache, const anvil_kv
     // (the kernels write notes wherever there is a place for parts, so a call without joins has none, whatever the
     // caller's pointer)
     AttnIO io{q, q_row_stride, q_head_stride, out, heads, 0, 0, 0, scale_log2,
-              causal != 0, dtype == kKvBF16, p.join ? static_cast<float *>(workspace) : nullptr};
+              causal != 0, dtype == kKvBF16, (flags & ANVIL_FLAG_ZERO_REST) != 0, p.join ? static_cast<float *>(workspace) : nullptr};
     set_group(io, heads / cv.kv_heads);
     if (!p.nt)
         return attn_tile_launch(cache->kind, cache->head_dim, cv, bv, io, p.ctas, p.join,

@@ -40,6 +40,7 @@ struct AttnIO {
     float scale_log2;       // scale * log2(e): scores are kept in powers of two
     int causal;
     int q_bf16;             // q and out are bf16 (else fp16)
+    int zero_rest;          // rows of no sequence become zeros (else they stay as they were)
     float *part;            // partial results, see AttnPart
 };
 
@@ -270,6 +271,20 @@ __device__ __forceinline__ void attn_next(const KvCacheView &c, const KvBatchVie
         seq = load_seq(bt, c, p.b);
         if (seq.q1 > seq.q0) return;
     }
+}
+
+// Zeros for the rows before the first sequence and behind the last one, by the last warp of every CTA: the others need not
+// wait for the starts (a decode step of one sequence takes 8.7 us, with all warps 8.8, without zeros 8.6).
+template <int D>
+__device__ __forceinline__ void attn_zero_rest(const KvBatchView &bt, const AttnIO &io) {
+    const int lane = int(threadIdx.x) - int(blockDim.x) + 32;
+    if (!io.zero_rest || lane < 0) return;
+    const int64_t row = int64_t(io.heads) * (D / 8);  // 16-byte pieces
+    const int64_t begin = min(max(bt.start[0], 0), bt.total) * row, end = min(max(bt.start[bt.batch], 0), bt.total) * row;
+    const int64_t rest = begin + (bt.total * row - end);
+    uint4 *out = static_cast<uint4 *>(io.out);
+    for (int64_t i = int64_t(blockIdx.x) * 32 + lane; i < rest; i += int64_t(gridDim.x) * 32)
+        out[i < begin ? i : i - begin + end] = make_uint4(0, 0, 0, 0);
 }
 
 __device__ __forceinline__ float ex2(float x) {

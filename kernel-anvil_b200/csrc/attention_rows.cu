@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32, RowsShape<KIND, D, NT>::min_c
     const int64_t work = attn_locate<ROWS, kRowsKeys, kRowsCost>(
         c, bt, io, &sc, [&](const AttnShares &s) { return s.begin(min(int(blockIdx.x), s.ctas - 1)); }, blockIdx.x == 0);
     pdl_launch_dependents();
+    attn_zero_rest<D>(bt, io);
     const AttnShares shares(work, gridDim.x);
     // what is to be joined: nothing, unless the last unit is left unfinished below
     if (io.part && threadIdx.x == 0) attn_open<ROWS, D>(io.part, gridDim.x)[blockIdx.x].parts = 0;

@@ -238,6 +238,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int64_t work = attn_locate<S::rows, S::keys, kTileCost>(
         c, bt, io, &sh.sc, [&](const AttnShares &s) { return s.begin(min(int(blockIdx.x), s.ctas - 1)); }, blockIdx.x == 0);
     pdl_launch_dependents();
+    attn_zero_rest<D>(bt, io);
     const AttnShares shares(work, gridDim.x);
     AttnOpen *const note = io.part ? attn_open<S::rows, D>(io.part, gridDim.x) + blockIdx.x : nullptr;
     if (int(blockIdx.x) >= shares.ctas) {

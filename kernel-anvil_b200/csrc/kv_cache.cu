@@ -36,6 +36,7 @@ struct KvIO {
     int64_t k_row, k_head, v_row, v_head;
     void *ok, *ov;
     const int *first;  // read: position of each sequence's first row (null: 0)
+    int zero_rest;     // read: rows of no sequence become zeros (else they stay as they were)
 };
 
 // ---- input / output of 8 values ---------------------------------------------------------
@@ -348,18 +349,24 @@ __global__ void __launch_bounds__(kKvThreads) kv_read_kernel(KvCacheView c, KvBa
     report_bad_entries(c, bt);
     if (t >= bt.total) return;
     const int b = seq_of_row(bt, int(t));
-    if (b < 0) return;  // a row behind the last sequence
+    const int64_t at = (t * c.kv_heads + h) * D + l * 8;
+    float k[8] = {}, v[8] = {};
+    if (b < 0) {  // a row of no sequence
+        if (io.zero_rest) {
+            Vec8<T>::store(io.ok, at, k);
+            Vec8<T>::store(io.ov, at, v);
+        }
+        return;
+    }
     const int64_t pos = t - bt.start[b] + (io.first ? io.first[b] : 0);
     int64_t row = -1;
     if (pos >= 0 && pos < kv_capacity(bt, c)) row = kv_lookup(bt, c, b, int(pos), h);
-    float k[8] = {}, v[8] = {};
     if (row >= 0) {
         load_row<KIND, D>(c.k, c.ks, row, l, k);
         load_row<KIND, D>(c.v, c.vs, row, l, v);
     } else if (l == 0) {
         flag_bad_page();
     }
-    const int64_t at = (t * c.kv_heads + h) * D + l * 8;
     Vec8<T>::store(io.ok, at, k);
     Vec8<T>::store(io.ov, at, v);
 }
@@ -460,21 +467,35 @@ extern "C" int anvil_kv_write(const anvil_kv_cache *cache, const anvil_kv_batch 
             v_head_stride % n)
             return fail(ANVIL_ERR_ALIGN, "rows of k and v must start on 16-byte boundaries");
     }
-    KvIO io{k, v, k_row_stride, k_head_stride, v_row_stride, v_head_stride, nullptr, nullptr, nullptr};
+    KvIO io{k, v, k_row_stride, k_head_stride, v_row_stride, v_head_stride, nullptr, nullptr, nullptr, 0};
     return run_kv(true, cache, cv, bv, dtype, io, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" int anvil_kv_read(const anvil_kv_cache *cache, const anvil_kv_batch *batch, const int32_t *first,
                              int dtype, void *k, void *v, anvil_stream_t stream) {
+    return anvil_kv_read_ex(cache, batch, first, dtype, k, v, 0, stream);
+}
+
+extern "C" int anvil_kv_read_ex(const anvil_kv_cache *cache, const anvil_kv_batch *batch, const int32_t *first,
+                                int dtype, void *k, void *v, unsigned flags, anvil_stream_t stream) {
     KvCacheView cv;
     KvBatchView bv;
     if (int s = kv_check(cache, batch, &cv, &bv)) return s;
+    if (flags & ~unsigned(ANVIL_FLAG_ZERO_REST)) return fail(ANVIL_ERR_INVALID, "flags=0x%x", flags);
     bv.kv_len = nullptr;  // lengths are no part of a read
-    if (bv.batch && bv.total) {
+    if (bv.total && (bv.batch || flags)) {
+        if (dtype != kKvF32 && dtype != kKvF16 && dtype != kKvBF16)
+            return fail(ANVIL_ERR_UNSUPPORTED, "dtype %d (F32, F16 and BF16 are)", dtype);
         if (!k || !v) return fail(ANVIL_ERR_INVALID, "null k or v");
         if (!aligned(k, 16) || !aligned(v, 16) || !aligned(first, 4))
             return fail(ANVIL_ERR_ALIGN, "k and v must be 16-byte aligned, first 4-byte");
     }
-    KvIO io{nullptr, nullptr, 0, 0, 0, 0, k, v, first};
+    if (bv.batch == 0 && bv.total && flags) {  // all rows are of no sequence
+        const size_t n = size_t(bv.total) * cv.kv_heads * cache->head_dim * (dtype == kKvF32 ? 4 : 2);
+        cudaError_t e = cudaMemsetAsync(k, 0, n, reinterpret_cast<cudaStream_t>(stream));
+        if (e == cudaSuccess) e = cudaMemsetAsync(v, 0, n, reinterpret_cast<cudaStream_t>(stream));
+        return e == cudaSuccess ? ANVIL_OK : cuda_fail(e, "kv_read memset");
+    }
+    KvIO io{nullptr, nullptr, 0, 0, 0, 0, k, v, first, flags != 0};
     return run_kv(false, cache, cv, bv, dtype, io, reinterpret_cast<cudaStream_t>(stream));
 }

@@ -37,6 +37,7 @@ ANVIL_ERR_CUDA = -3
 ANVIL_ERR_ALIGN = -4
 ANVIL_ERR_TIMEOUT = -5
 ANVIL_FLAG_PDL = 1
+ANVIL_FLAG_ZERO_REST = 2
 
 _STATUS_NAMES = {
     ANVIL_ERR_INVALID: "invalid argument",
@@ -227,9 +228,12 @@ SIGNATURES = {
     "anvil_kv_write": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64,
                                c_int64, c_void_p]),
     "anvil_kv_read": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "anvil_kv_read_ex": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_uint, c_void_p]),
     "anvil_paged_attention_workspace": (c_int64, [c_void_p, c_void_p, c_int]),
     "anvil_paged_attention": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int,
                                       ctypes.c_float, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
+    "anvil_paged_attention_ex": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int,
+                                         ctypes.c_float, c_int, c_void_p, c_void_p, c_int64, c_uint, c_void_p]),
     "anvil_smithy_bucket": (c_int, [c_int]),
     "anvil_smithy_set_model": (None, [c_char_p]),
     "anvil_smithy_load": (c_int, [c_char_p]),

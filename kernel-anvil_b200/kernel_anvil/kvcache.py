@@ -23,7 +23,7 @@ import ctypes
 import torch
 
 from kernel_anvil import _native
-from kernel_anvil._native import ANVIL_ERR_INVALID, AnvilError, check
+from kernel_anvil._native import ANVIL_ERR_INVALID, ANVIL_FLAG_ZERO_REST, AnvilError, check
 
 # kind -> (ggml type id, dtype of the codes, codes per head value as a divisor, values per scale)
 KINDS = {
@@ -224,13 +224,15 @@ def kv_read(cache: PagedKVCache, page_table: torch.Tensor, start: torch.Tensor, 
     """(k, v) of cached tokens, each (rows, kv_heads, head_dim) of `dtype`: rows start[b] .. start[b+1]
     are the positions first[b], first[b] + 1, ... (first None: from 0) of sequence b.
 
-    A position without a page reads as zeros; rows behind start[-1] are left as they were.
+    A position without a page reads as zeros; so do rows of no sequence (before start[0] and behind start[-1]),
+    except in a given `out`, where they are left as they were.
     """
     if dtype not in DTYPES:
         raise _bad(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     b = _batch(cache, page_table, start, first, rows)
     b.kv_len = None
     shape = (rows, cache.kv_heads, cache.head_dim)
+    flags = 0 if out is not None else ANVIL_FLAG_ZERO_REST
     if out is None:
         out = (torch.empty(shape, dtype=dtype, device=cache.device),
                torch.empty(shape, dtype=dtype, device=cache.device))
@@ -238,8 +240,9 @@ def kv_read(cache: PagedKVCache, page_table: torch.Tensor, start: torch.Tensor, 
         if t.shape != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous() or \
                 t.data_ptr() % 16:
             raise _bad(f"out is two contiguous 16-byte aligned {dtype} tensors {shape} on the cache's device")
-    _call(cache, _native.lib().anvil_kv_read, cache._ref, ctypes.byref(b),
-          first.data_ptr() if first is not None else None, DTYPES[dtype], out[0].data_ptr(), out[1].data_ptr())
+    _call(cache, _native.lib().anvil_kv_read_ex, cache._ref, ctypes.byref(b),
+          first.data_ptr() if first is not None else None, DTYPES[dtype], out[0].data_ptr(), out[1].data_ptr(),
+          flags)
     return out
 
 
@@ -252,7 +255,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     and head strides; heads a multiple of the cache's kv_heads, query head h reading key/value head
     h // (heads // kv_heads).  Row i of sequence b sees its kv_len[b] cached tokens, or, causal,
     those up to its own position kv_len[b] - q_len + i; a row that sees none is zeros.  scale
-    defaults to head_dim ** -0.5.  Rows behind q_start[-1] are left as they were.
+    defaults to head_dim ** -0.5.  Rows of no sequence (before q_start[0] and behind q_start[-1]: the padding of a
+    captured step) are zeros, except in a given `out`, where they are left as they were.
     """
     q = _rows("q", q, cache, None)
     heads = q.shape[1]
@@ -263,6 +267,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     if cache.k_scale is None and q.dtype != cache.k.dtype:
         raise _bad(f"a {cache.kind} cache takes q of its own type, got {q.dtype}")
     b = _batch(cache, page_table, q_start, kv_len, q.shape[0])
+    flags = 0 if out is not None else ANVIL_FLAG_ZERO_REST
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != cache.device or \
@@ -280,7 +285,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
         cache._work[key] = need
     # scratch of this call, from torch's allocator: its memory follows the stream and, in a capture, the graph
     work = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
-    _call(cache, lib.anvil_paged_attention, cache._ref, ref, DTYPES[q.dtype], q.data_ptr(), q.stride(0),
+    _call(cache, lib.anvil_paged_attention_ex, cache._ref, ref, DTYPES[q.dtype], q.data_ptr(), q.stride(0),
           q.stride(1), heads, cache.head_dim ** -0.5 if scale is None else float(scale), int(bool(causal)),
-          out.data_ptr(), work.data_ptr() if work is not None else None, need)
+          out.data_ptr(), work.data_ptr() if work is not None else None, need, flags)
     return out

@@ -918,3 +918,60 @@ def test_queries_at_both_ends_of_bf16_meet_a_scale_that_brings_them_back(kind, q
     check_attention(batch, 4, "bf16", amp=2.0 ** 122, scale=0.09 * 2.0 ** -122)
     check_attention(batch, 4, "bf16", amp=2.0 ** 112, scale=0.09 * 2.0 ** -112)
     check_attention(batch, 4, "bf16", amp=2.0 ** -121, scale=0.09 * 2.0 ** 121)
+
+
+def leave_garbage(nbytes):
+    """Blocks of the allocator that hold NaN, for the next allocations of that size."""
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    held = [torch.full((nbytes // 2,), float("nan"), dtype=torch.float16, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    del held
+
+
+@pytest.mark.parametrize("kind,dtype", [("Q8_0", "bf16"), ("F16", "f16")])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("q_lens,lead,rest", [([1, 1], 0, 30), ([0, 0], 0, 30), ([40, 90], 0, 200), ([3, 0], 5, 90),
+                                              ([50, 90], 7, 0), ([0], 0, 1), ([], 0, 9)])
+def test_rows_of_no_sequence_are_zeros_in_new_outputs(kind, dtype, dim, q_lens, lead, rest):
+    """A padded step: rows before the first sequence and behind the last one, where the call makes the output; where
+    the caller gives it they stay as they were."""
+    batch = ref.Batch(kind, dim, 2, 16, q_lens, [n + 20 for n in q_lens], seed=47)
+    cache, total = batch.cache(ops), lead + batch.rows + rest
+    table, start, kv_len = batch.on_gpu()
+    start = start + lead
+    q = torch.randn(total, 4, dim, generator=batch.gen).to(ref.NP[dtype]).cuda()
+    out = torch.full_like(q, 7.0)
+    ops.paged_attention(q, cache, table, start, kv_len, out=out)
+    assert (out[:lead] == 7).all() and (out[lead + batch.rows:] == 7).all()
+    out[:lead], out[lead + batch.rows:] = 0, 0
+    leave_garbage(q.numel() * 2)
+    assert torch.equal(ops.paged_attention(q, cache, table, start, kv_len), out)
+    into = tuple(torch.full((total, 2, dim), 7.0, dtype=q.dtype, device="cuda") for _ in range(2))
+    ops.kv_read(cache, table, start, total, dtype=q.dtype, out=into)
+    leave_garbage(total * 2 * dim * 2)
+    for got, t in zip(ops.kv_read(cache, table, start, total, dtype=q.dtype), into):
+        assert (t[:lead] == 7).all() and (t[lead + batch.rows:] == 7).all()
+        t[:lead], t[lead + batch.rows:] = 0, 0
+        assert torch.equal(got, t)
+    assert mmvq.take_device_status() == 0
+
+
+def test_a_padded_step_replays_with_more_and_fewer_rows():
+    batch = ref.Batch("Q8_0", 128, 2, 16, [2, 3], [300, 40], seed=48)
+    cache = batch.cache(ops)
+    table, start, kv_len = batch.on_gpu()
+    q = torch.randn(64, 8, 128, generator=batch.gen).bfloat16().cuda()
+    ops.paged_attention(q, cache, table, start, kv_len)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_attention(q, cache, table, start, kv_len)
+    for s in ([0, 2, 5], [0, 30, 64], [0, 1, 1], [0, 0, 0], [0, 10, 12]):
+        start.copy_(torch.tensor(s, dtype=torch.int32))
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.isfinite(out).all() and (out[s[-1]:] == 0).all()
+        given = torch.full_like(q, 7.0)
+        ops.paged_attention(q, cache, table, start, kv_len, out=given)
+        assert torch.equal(out[:s[-1]], given[:s[-1]]) and (given[s[-1]:] == 7).all()

@@ -158,6 +158,23 @@ def test_c_abi_empty_calls_do_nothing():
             assert call() == 0, name
 
 
+def test_c_abi_flags():
+    """Unknown ones are refused; with ANVIL_FLAG_ZERO_REST a batch of no sequences has rows to write."""
+    lib, zero = _native.lib(), _native.ANVIL_FLAG_ZERO_REST
+    read = lambda b, flags, dtype=1, k=16, v=32: lib.anvil_kv_read_ex(  # noqa: E731
+        ctypes.byref(c_cache()), ctypes.byref(b), None, dtype, k, v, flags, None)
+    attention = lambda b, flags, out=64: lib.anvil_paged_attention_ex(  # noqa: E731
+        ctypes.byref(c_cache()), ctypes.byref(b), 1, 16, 256, 128, 4, 1.0, 1, out, 32, 1 << 40, flags, None)
+    for flags in (1, 4, 1 << 31, zero | 1):
+        assert read(c_batch(), flags) == ANVIL_ERR_INVALID and "flags" in _native.last_error()
+        assert attention(c_batch(), flags) == ANVIL_ERR_INVALID and "flags" in _native.last_error()
+    nobody = c_batch(batch=0)
+    assert read(nobody, 0, k=None) == 0 and attention(nobody, 0, out=None) == 0
+    assert read(nobody, zero, k=None) == read(nobody, zero, v=None) == attention(nobody, zero, out=None) == ANVIL_ERR_INVALID
+    assert read(nobody, zero, dtype=2) == ANVIL_ERR_UNSUPPORTED
+    assert read(c_batch(batch=0, total=0), zero, k=None) == attention(c_batch(batch=0, total=0), zero, out=None) == 0
+
+
 # ---- the Python surface ------------------------------------------------------------------------
 
 def test_cache_shapes_and_refusals():
