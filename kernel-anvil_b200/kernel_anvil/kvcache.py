@@ -240,6 +240,8 @@ def kv_read(cache: PagedKVCache, page_table: torch.Tensor, start: torch.Tensor, 
         if t.shape != shape or t.dtype != dtype or t.device != cache.device or not t.is_contiguous() or \
                 t.data_ptr() % 16:
             raise _bad(f"out is two contiguous 16-byte aligned {dtype} tensors {shape} on the cache's device")
+    if abs(out[0].data_ptr() - out[1].data_ptr()) < out[0].numel() * out[0].element_size():
+        raise _bad("the two tensors of out overlap")
     _call(cache, _native.lib().anvil_kv_read_ex, cache._ref, ctypes.byref(b),
           first.data_ptr() if first is not None else None, DTYPES[dtype], out[0].data_ptr(), out[1].data_ptr(),
           flags)

@@ -975,3 +975,15 @@ def test_a_padded_step_replays_with_more_and_fewer_rows():
         given = torch.full_like(q, 7.0)
         ops.paged_attention(q, cache, table, start, kv_len, out=given)
         assert torch.equal(out[:s[-1]], given[:s[-1]]) and (given[s[-1]:] == 7).all()
+
+
+def test_a_read_into_overlapping_buffers_is_refused():
+    batch = ref.Batch("Q8_0", 64, 2, 16, [5], [5], seed=50)
+    table, start, _ = batch.on_gpu()
+    cache, both = batch.cache(ops), torch.zeros(11, 2, 64, device="cuda")
+    for out in ((both[:5], both[:5]), (both[:5], both[4:9]), (both[4:9], both[:5])):
+        with pytest.raises(AnvilError, match="overlap"):
+            ops.kv_read(cache, table, start, 5, out=out)
+    ops.kv_read(cache, table, start, 5, out=(both[5:10], both[:5]))
+    assert torch.equal(both[5:10].cpu(), batch.rows_of("k", 0).float())
+    assert mmvq.take_device_status() == 0
