@@ -258,7 +258,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     h // (heads // kv_heads).  Row i of sequence b sees its kv_len[b] cached tokens, or, causal,
     those up to its own position kv_len[b] - q_len + i; a row that sees none is zeros.  scale
     defaults to head_dim ** -0.5.  Rows of no sequence (before q_start[0] and behind q_start[-1]: the padding of a
-    captured step) are zeros, except in a given `out`, where they are left as they were.
+    captured step) are zeros, except in a given `out`, where they are left as they were.  out may be q itself, but not
+    overlap it otherwise.
     """
     q = _rows("q", q, cache, None)
     heads = q.shape[1]
@@ -275,6 +276,11 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != cache.device or \
             not out.is_contiguous() or out.data_ptr() % 16:
         raise _bad("out is a contiguous 16-byte aligned tensor of q's shape and type on the cache's device")
+    elif out.numel() and not (out.data_ptr() == q.data_ptr() and q.is_contiguous()):  # (q itself is: rows are read first)
+        span = 1 + sum((n - 1) * step for n, step in zip(q.shape, q.stride()))
+        at = (out.data_ptr() - q.data_ptr()) // q.element_size()
+        if -out.numel() < at < span:
+            raise _bad("out overlaps q without being q")
     if kv_len is None:
         raise _bad("kv_len is needed")
     lib, ref = _native.lib(), ctypes.byref(b)

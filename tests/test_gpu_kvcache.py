@@ -987,3 +987,26 @@ def test_a_read_into_overlapping_buffers_is_refused():
     ops.kv_read(cache, table, start, 5, out=(both[5:10], both[:5]))
     assert torch.equal(both[5:10].cpu(), batch.rows_of("k", 0).float())
     assert mmvq.take_device_status() == 0
+
+
+@pytest.mark.parametrize("kind,dtype", [("Q8_0", "bf16"), ("F16", "f16")])
+@pytest.mark.parametrize("q_lens", [[1, 4], [60, 250]])
+def test_attention_in_place_and_over_parts_of_its_queries(kind, dtype, q_lens):
+    batch = ref.Batch(kind, 128, 2, 16, q_lens, [3000, 900], seed=52)
+    cache, n = batch.cache(ops), batch.rows
+    table, start, kv_len = batch.on_gpu()
+    room = torch.zeros(2 * n + 1, 4, 128, dtype=ref.NP[dtype], device="cuda")
+    q = make_q(batch, 4, dtype)
+    want = ops.paged_attention(q, cache, table, start, kv_len)
+    for at in (1, n - 1):
+        for a, b in ((0, at), (at, 0)):
+            room[a:a + n] = q
+            with pytest.raises(AnvilError, match="overlap"):
+                ops.paged_attention(room[a:a + n], cache, table, start, kv_len, out=room[b:b + n])
+    wide = torch.zeros(n, 8, 128, dtype=q.dtype, device="cuda")
+    with pytest.raises(AnvilError, match="overlap"):    # a strided view that starts where out does
+        ops.paged_attention(wide[:, :4], cache, table, start, kv_len, out=wide.view(-1)[:n * 512].view(n, 4, 128))
+    room[:n] = q
+    assert torch.equal(ops.paged_attention(room[:n], cache, table, start, kv_len, out=room[n:2 * n]), want)
+    assert torch.equal(ops.paged_attention(room[:n], cache, table, start, kv_len, out=room[:n]), want)
+    assert mmvq.take_device_status() == 0
