@@ -177,6 +177,8 @@ def _rows(name: str, x: torch.Tensor, cache: PagedKVCache, heads: int | None) ->
         raise _bad(f"{name} must be float32, float16 or bfloat16, got {x.dtype}")
     if x.requires_grad and torch.is_grad_enabled():
         raise _bad(f"{name} requires grad, and the cache's operators have no backward pass")
+    if torch.autograd.forward_ad.unpack_dual(x).tangent is not None:
+        raise _bad(f"{name} carries a tangent, and the cache's operators have no forward-mode derivative")
     row, head, inner = x.stride()
     n = 4 if x.dtype == torch.float32 else 8  # values in 16 bytes
     if inner != 1 or row % n or head % n or x.data_ptr() % 16:

@@ -208,6 +208,28 @@ def test_no_cpu_path():
             call()
 
 
+def test_inputs_of_either_differentiation_are_refused():
+    """Neither a gradient nor a tangent is dropped silently (refused before anything else, so no GPU is needed)."""
+    from torch.autograd import forward_ad
+
+    batch = ref.Batch("F16", 64, 2, 16, [3], [20])
+    cache = kvcache.PagedKVCache.from_buffers("F16", batch.k, batch.v)
+    args = (batch.table, batch.start, batch.kv_len)
+    x = torch.randn(3, 2, 64).half()
+    with pytest.raises(AnvilError, match="backward"):
+        kvcache.paged_attention(x.clone().requires_grad_(), cache, *args)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: kvcache.paged_attention(dual, cache, *args), lambda: kvcache.kv_write(cache, dual, x, *args),
+                     lambda: kvcache.kv_write(cache, x, dual, *args)):
+            with pytest.raises(AnvilError, match="forward-mode"):
+                call()
+        with pytest.raises(AnvilError, match="no CPU path"):    # others pass this check
+            kvcache.paged_attention(x, cache, *args)
+    with torch.no_grad(), pytest.raises(AnvilError, match="no CPU path"):
+        kvcache.paged_attention(x.clone().requires_grad_(), cache, *args)
+
+
 def test_rules_are_the_gguf_types():
     """Codes and scales of the oracle (which the GPU tests hold the kernels to) against gguf-py's blocks:
     equal but where a value stands within fp32 rounding of a border."""
