@@ -186,17 +186,15 @@ def _rows(name: str, x: torch.Tensor, cache: PagedKVCache, heads: int | None) ->
     return x
 
 
-_stream = torch._C._cuda_getCurrentRawStream  # of a device index, without the Stream object
-
-
 def _call(cache: PagedKVCache, fn, *args) -> None:
     """fn(*args, stream) on the cache's device and torch's current stream there."""
     index = cache.device.index
-    if index == torch._C._cuda_getDevice():
-        status = fn(*args, _stream(index))
+    stream = torch.cuda.current_stream(index).cuda_stream
+    if index == torch.cuda.current_device():
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(index):
-            status = fn(*args, _stream(index))
+            status = fn(*args, stream)
     if status < 0:
         check(status)
 

@@ -208,6 +208,29 @@ def test_no_cpu_path():
             call()
 
 
+def test_the_module_needs_nothing_of_a_torch_with_cuda_to_be_imported():
+    """A torch built without CUDA lacks torch._C's CUDA functions: the import still works, and calls are refused."""
+    import os
+    import sys
+
+    code = """
+import torch
+for name in [n for n in dir(torch._C) if n.startswith("_cuda_")]:
+    delattr(torch._C, name)
+from kernel_anvil import kvcache
+cache = kvcache.PagedKVCache(5, 16, 2, 128, "F16", device="cpu")
+table, start = torch.zeros(1, 5, dtype=torch.int32), torch.tensor([0, 3], dtype=torch.int32)
+try:
+    kvcache.kv_read(cache, table, start, 3)
+except kvcache.AnvilError as e:
+    assert "no CPU path" in str(e)
+else:
+    raise SystemExit(1)
+"""
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(p for p in sys.path if p))
+    subprocess.run([sys.executable, "-c", code], check=True, env=env, timeout=300)
+
+
 def test_inputs_of_either_differentiation_are_refused():
     """Neither a gradient nor a tangent is dropped silently (refused before anything else, so no GPU is needed)."""
     from torch.autograd import forward_ad
