@@ -433,7 +433,7 @@ int anvil_kv_read_ex(const anvil_kv_cache *cache, const anvil_kv_batch *batch, c
 
 /* out[t][h] = sum_j softmax_j(scale q[t][h] . k_j) v_j over the cached tokens j that the row
  * sees: all kv_len[b] of its sequence, or, causal, those up to its own position; zeros for a
- * row that sees none.  Query head h reads key/value head h / (heads / kv_heads).  q: dtype 1
+ * row that sees none, or none with a score above -infinity.  Query head h reads key/value head h / (heads / kv_heads).  q: dtype 1
  * or 30, for an F16 / BF16 cache the cache's own; strides in values, 16-byte aligned rows; out:
  * (total, heads, head_dim), contiguous, of q's type.  Keys without a page are left out.  What
  * lies behind kv_len in a page is never used; keys that a row does not see do not reach it, NaN

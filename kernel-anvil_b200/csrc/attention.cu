@@ -32,6 +32,9 @@ int attn_take_status() {
 
 // The grid: every resident slot, or fewer where the batch cannot have that many key tiles.  It
 // follows from the batch's outer sizes, not from lengths, which are on the device.
+// (A constant, so that the workspace can be asked for without a device and the order of the sums is the same on every one; on
+// a part with fewer multiprocessors the CTAs take turns.)
+constexpr int kAttnSms = 148;
 struct AttnPlan {
     int nt;         // row tile of the rows kernel in eighths; 0: the tile kernel
     int ctas;
@@ -58,7 +61,7 @@ static AttnPlan attn_plan(const anvil_kv_cache *c, const KvCacheView &cv, const 
     const int64_t capacity = kv_capacity(bv, cv);
     const int64_t units = int64_t(cv.kv_heads) * (int64_t(bv.total) * group / t.rows + std::min(bv.batch, bv.total));
     const int64_t per = std::max<int64_t>(1, (capacity + t.keys - 1) / t.keys);
-    const int64_t slots = 148 * t.occ;
+    const int64_t slots = int64_t(kAttnSms) * t.occ;
     p.ctas = int(per > slots / std::max<int64_t>(units, 1) ? slots : std::min(slots, units * per));
     p.join = per > 1;
     p.bytes = p.join ? (int64_t(t.rows) * (c->head_dim + 2) * 8 + int64_t(sizeof(AttnOpen))) * p.ctas : 0;

@@ -4,13 +4,16 @@
 // Arithmetic: mma.sync m16n8k16 with fp32 sums, transposed so that the keys, not the few queries,
 // fill the 16 rows of a product: S^T = K Q^T (16 keys x 8 queries), then the weights by a reference that
 // is raised when one grows large, and their sum, then O^T += V^T P^T.  P is rounded to the products' 16-bit type (fp16
-// 2^-11, bf16 2^-8 of each weight) and a quantised value to fp16 (2^-11): the products take 16 bits; scores,
-// references, sums and outputs are fp32.  A tile of 8 queries costs half the products, exponentials and
-// registers that a 16-row tile of queries would, and widening the codes, which dominates, is done once
-// for all queries.  The legacy tensor path is enough: it works a fifth of the time at the rate at which
+// 2^-11, bf16 2^-8 of each weight) and a quantised value to fp16 (2^-11).  That is a choice: the tensor cores' floats
+// have no more bits than fp16's, and operands in two halves would take two or three products for each.  With fp16
+// outputs the error against 64 bits is then 3.4e-4 of the outputs' norm, where their own rounding is 2.1e-4.  Scores of
+// quantised keys are of exact codes; scores, references, sums and outputs are fp32.  A tile of 8 queries costs half the
+// products, exponentials and registers that a 16-row tile of queries would, and widening the codes, which dominates, is
+// done once for all queries.  The legacy tensor path is enough: it works a fifth of the time at the rate at which
 // HBM delivers keys, and tcgen05's smallest tile has 64 rows, of which a decode step fills 8.
 //
-// What bounds it: 48 sequences of 300 to 9000 tokens in Q8_0 (573 MB) take 114 us, 77% of the measured HBM rate.  Q4_0
+// What bounds it: 48 sequences of 300 to 9000 tokens in Q8_0 (573 MB) take 115 us, 76% of the measured HBM rate, and 124 to 129
+// once it has run for some milliseconds, when the card's 1000 W cap holds its clock (1725 MHz).  Q4_0
 // carries twice the values a byte, and there the instructions that widen them bound it: one row over 120000
 // keys (138 MB) takes 64 us, 33%, of which some 8 are the join and the launches.  A decode step of 4 short
 // sequences takes 9 us, which is latency: finding its share, one ring, the join.

@@ -20,11 +20,15 @@
 // Weights are taken by a reference, which a row's first tile sets near its maximum; it is raised, and O rescaled,
 // only when a tile's weights sum to more than fp16 holds, which the sum that is taken anyway shows: most tiles are
 // never searched for their maximum.  P is rounded to the products' 16-bit type (fp16 2^-11, bf16 2^-8 of each weight) and
-// quantised keys and values to fp16 (2^-11), since the products take 16 bits; scores, sums and outputs are fp32.
+// quantised keys and values to fp16 (2^-11); scores, sums and outputs are fp32.  That is a choice: the tensor cores' floats
+// have no more bits than fp16's (tf32 rounds alike), P has V's type, as the instruction wants it, and operands in two halves
+// would take two or three products for each.  With fp16 outputs the error against 64 bits is 2 to 3 times the output's own
+// rounding (5.7e-4 against 2.1e-4, Q8_0), with a BF16 cache 1.3 times (2.1e-3 against 1.6e-3).
 //
 // What bounds it: the softmax, some 2000 cycles for the 64 keys of 256 rows (64 exponentials, as many roundings and the moves
-// from and to tensor memory a thread, four warps a scheduler); the products take about 1300.  7993 rows of 64 heads of 128 over themselves, BF16,
-// take 0.55 ms, 950 TFLOP/s or 57% of the measured GEMM rate; 2048 over 30049 keys of Q8_0 2.19 ms, 890 TFLOP/s.
+// from and to tensor memory a thread, four warps a scheduler); the products take about 1300.  No pipe is full
+// (tcgen05 59%, exponentials 50%, issue slots 39%): the two wait for one another.  7993 rows of 32 heads of 128 over themselves, BF16,
+// take 0.55 ms, 950 TFLOP/s or 57% of the measured GEMM rate; 2048 rows of 64 heads over 30049 keys of Q8_0 2.2 ms, 880 TFLOP/s.
 // Short sequences pay kTileCost for each unit: 12 sequences of 1 to 600 new tokens 0.36 ms, 490 TFLOP/s.
 #include <cuda.h>
 

@@ -260,7 +260,8 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     q: (rows, heads, head_dim), float16 or bfloat16 (an F16 / BF16 cache takes its own type), any row
     and head strides; heads a multiple of the cache's kv_heads, query head h reading key/value head
     h // (heads // kv_heads).  Row i of sequence b sees its kv_len[b] cached tokens, or, causal,
-    those up to its own position kv_len[b] - q_len + i; a row that sees none is zeros.  scale
+    those up to its own position kv_len[b] - q_len + i; a row that sees none (or whose scores are all -inf)
+    is zeros.  scale
     defaults to head_dim ** -0.5.  Rows of no sequence (before q_start[0] and behind q_start[-1]: the padding of a
     captured step) are zeros, except in a given `out`, where they are left as they were.  out may be q itself, but not
     overlap it otherwise.
